@@ -181,10 +181,10 @@ def _run_own(st):
             return {"loss": loss, "lse": lse}
         dH, dW, db = dgx.linear_nll_bwd(H, W, st["target"], lse, bias=b, dloss=st["dloss"], scale=st["scale"])
     else:
-        loss, lse, zsel = dgx.linear_distill_fwd(H, W, st["idx"], st["teacher"], bias=b, temperature=c["T"])
+        loss, lse = dgx.linear_distill_fwd(H, W, st["idx"], st["teacher"], bias=b, temperature=c["T"])
         if not c["train"]:
             return {"loss": loss, "lse": lse}
-        dH, dW, db = dgx.linear_distill_bwd(H, W, st["idx"], st["teacher"], lse, zsel, bias=b, temperature=c["T"],
+        dH, dW, db = dgx.linear_distill_bwd(H, W, st["idx"], st["teacher"], lse, bias=b, temperature=c["T"],
                                             scale=st["scale"])
     return {"loss": loss, "lse": lse, "dH": dH, "dW": dW, "db": db}
 

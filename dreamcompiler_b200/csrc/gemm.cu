@@ -605,7 +605,11 @@ static cudaError_t launch_tc_bn(const GemmArgs& args, const void* A, const void*
     const int tiles = a.tiles_m * a.tiles_n;
     const int nk_all = (args.K + Cfg::BK - 1) / Cfg::BK;
     if (a.n_extra == 0 && nb == 1 && tiles * 2 <= num_sms() && nk_all >= 16) {
-      const int sp = std::min(std::min(num_sms() / tiles, nk_all / 8), 16);
+      int sp = std::min(std::min(num_sms() / tiles, nk_all / 8), 16);
+      if (sp >= 2) {  // no empty slice: the kernel's slices are ceil(nk_all / splits) blocks long
+        const int kper = (nk_all + sp - 1) / sp;
+        sp = (nk_all + kper - 1) / kper;
+      }
       ldw = (a.N + 3) & ~3;
       if (sp >= 2 && (ws = (float*)library_scratch_slot(kScratchSplitK, (size_t)sp * a.M * ldw * sizeof(float), stream)) !=
               nullptr)

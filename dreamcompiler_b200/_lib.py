@@ -80,6 +80,17 @@ SIGNATURES = {
     "dgx_colsum": (_i, [_vp, _i, _vp, _i, _i, _i, _vp]),
     "dgx_rows_to_heads": (_i, [_vp, _i, _i, _i, _vp, _i, _i, _i, _i, _vp]),
     "dgx_heads_to_rows": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "dgx_linear_nll_fwd": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "dgx_linear_nll_bwd": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _vp, _i, _i, _vp, _i, _i, _vp, _i,
+                                _vp, _sz, _vp]),
+    "dgx_linear_nll_workspace_size": (_sz, [_i] * 4),
+    "dgx_linear_distill_fwd": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _f, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "dgx_linear_distill_bwd": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _f, _vp, _vp, _f, _i, _i, _i, _vp, _i, _i, _vp,
+                                    _i, _i, _vp, _i, _vp, _sz, _vp]),
+    "dgx_linear_distill_workspace_size": (_sz, [_i] * 5),
+    "dgx_embed_fwd": (_i, [_vp, _vp, _i, _i, _vp, _i, _f, _vp, _i, _i, _i, _i, _i, _vp]),
+    "dgx_embed_bwd": (_i, [_vp, _vp, _i, _i, _f, _vp, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "dgx_embed_bwd_workspace_size": (_sz, [_i] * 3),
     "dgx_tp_shard": (None, [_i, _i, _i, C.POINTER(_i), C.POINTER(_i)]),
     "dgx_tp_export": (_i, [_vp, _sz, _vp, _sz]),
     "dgx_tp_handle_size": (_sz, []),

@@ -1,0 +1,45 @@
+// Internal interface of the vocabulary-head kernels (linear + softmax losses
+// that never keep the logits): head.cu runs what head_api.cu has validated.
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "common.h"
+
+namespace dgx {
+
+constexpr int kHeadMaxK = 256;  // teacher entries per row
+
+// One problem: logits z = (H . W^T + bias) / T of R rows over V columns, and a
+// sparse target per row: K ids with K probabilities. The hard target is K = 1
+// with probability 1 and teacher == nullptr.
+struct HeadArgs {
+  const void* H;       // [R][ldh] bf16
+  const void* W;       // [V][ldw] bf16
+  const float* bias;   // [V] or null
+  const int* idx;      // [R][K]; an id outside [0, V) is an absent entry
+  const float* teacher;  // [R][K] teacher logits, or null (hard target)
+  int ldh, ldw, R, V, d, K;
+  float t, inv_t;      // temperature and its reciprocal
+  // forward results (inputs of the backward)
+  float* loss;         // [R]
+  float* lse;          // [R] log-sum-exp of z
+  float* mean;         // sum of loss / R, or null
+  // backward
+  const float* dloss;  // [R] weight per row, or null (1)
+  float scale;
+  void* dH;            // [R][lddh] or null
+  void* dW;            // [V][lddw] or null
+  float* db;           // [V] or null
+  int dh_bf16, lddh, dw_bf16, lddw;
+  int accumulate;      // dW (fp32) and db are added to
+  uint32_t* err;
+};
+
+size_t head_fwd_scratch_bytes(int R, int V, int d, int K, bool lists);
+size_t head_bwd_scratch_bytes(int R, int V, int d, int K, bool lists);
+dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s);
+dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s);
+
+}  // namespace dgx

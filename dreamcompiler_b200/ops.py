@@ -236,6 +236,189 @@ def quantize_rows_i8(X: torch.Tensor):
     return Xq, sx
 
 
+def linear_nll_workspace_size(R: int, V: int, d: int, backward: bool) -> int:
+    return L.load().dgx_linear_nll_workspace_size(R, V, d, int(backward))
+
+
+def linear_distill_workspace_size(R: int, V: int, d: int, K: int, backward: bool) -> int:
+    return L.load().dgx_linear_distill_workspace_size(R, V, d, K, int(backward))
+
+
+def _ws(workspace: Optional[torch.Tensor]):
+    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+
+
+def _head_check(H, W, bias, rows32, rowsf):
+    """Shapes and types shared by the vocabulary-head wrappers; returns (R, V, d)."""
+    assert H.is_cuda and H.dtype == torch.bfloat16 and H.dim() == 2 and H.stride(1) == 1, "H: [R, d] bf16 CUDA rows"
+    assert W.device == H.device and W.dtype == torch.bfloat16 and W.dim() == 2 and W.stride(1) == 1, "W: [V, d] bf16 rows"
+    (R, d), V = H.shape, W.shape[0]
+    assert W.shape[1] == d, f"H has {d} columns, W {W.shape[1]}"
+    if bias is not None:
+        assert bias.device == H.device and bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == V
+    assert rows32.device == H.device and rows32.dtype == torch.int32 and rows32.is_contiguous() and rows32.shape[0] == R
+    for t in rowsf:
+        if t is not None:
+            assert t.device == H.device and t.dtype == torch.float32 and t.is_contiguous() and t.shape[0] == R
+    return R, V, d
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Row pitch in elements. torch reports any stride for a single row."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
+
+
+def _grad_out(out, want: bool, rows: int, d: int, dtype, device):
+    """The tensor a gradient goes to: the caller's, a new one (rows padded to 16 bytes), or None."""
+    if not want:
+        return None
+    if out is None:
+        dp = (d + 7) // 8 * 8
+        out = torch.empty(rows, dp, device=device, dtype=dtype)
+        return out if dp == d else out[:, :d]
+    assert out.device == device and out.shape == (rows, d) and (out.stride(1) == 1 or d == 1) and out.dtype in _DT
+    return out
+
+
+def linear_nll_fwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+                   loss: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                   mean: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
+    """Negative log-likelihood of `target` under softmax(H W^T + bias), without
+    keeping the logits. H [R, d] bf16, W [V, d] bf16, bias [V] fp32, target [R]
+    int32 (outside [0, V): no target, loss 0). Returns (loss [R], lse [R]), the
+    row log-sum-exp being what linear_nll_bwd needs; `mean` (one fp32 element)
+    receives sum(loss) / R."""
+    R, V, d = _head_check(H, W, bias, target, (loss, lse))
+    assert target.dim() == 1
+    if loss is None:
+        loss = torch.empty(R, device=H.device, dtype=torch.float32)
+    if lse is None:
+        lse = torch.empty(R, device=H.device, dtype=torch.float32)
+    ws, wsb = _ws(workspace)
+    L.call("dgx_linear_nll_fwd", H.data_ptr(), _pitch(H), W.data_ptr(), _pitch(W), _ptr(bias), target.data_ptr(), R, V,
+           d, loss.data_ptr(), lse.data_ptr(), _ptr(mean), ws, wsb, _stream(H))
+    return loss, lse
+
+
+def linear_nll_bwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, *,
+                   bias: Optional[torch.Tensor] = None, dloss: Optional[torch.Tensor] = None, scale: float = 1.0,
+                   dH: Optional[torch.Tensor] = None, dW: Optional[torch.Tensor] = None,
+                   db: Optional[torch.Tensor] = None, need=("dH", "dW", "db"), accumulate: bool = False,
+                   workspace: Optional[torch.Tensor] = None):
+    """Gradients of sum_r scale * dloss[r] * loss[r] (dloss None: 1). Returns
+    (dH [R, d], dW [V, d], db [V] fp32); those not in `need` (and db without a
+    bias) are None. dH and dW are new bf16 tensors unless given (bf16 or fp32);
+    accumulate adds to the given fp32 dW and db."""
+    R, V, d = _head_check(H, W, bias, target, (lse, dloss))
+    dH, dW, db = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate)
+    ws, wsb = _ws(workspace)
+    L.call("dgx_linear_nll_bwd", H.data_ptr(), _pitch(H), W.data_ptr(), _pitch(W), _ptr(bias), target.data_ptr(),
+           lse.data_ptr(), _ptr(dloss), float(scale), R, V, d, *_grad_args(dH), *_grad_args(dW), _ptr(db),
+           int(accumulate), ws, wsb, _stream(H))
+    return dH, dW, db
+
+
+def _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate):
+    assert not accumulate or (("dW" not in need or dW is not None) and ("db" not in need or bias is None or db is not None)), \
+        "accumulate needs the tensors to add to"
+    dH = _grad_out(dH, "dH" in need, R, d, torch.bfloat16, H.device)
+    dW = _grad_out(dW, "dW" in need, V, d, torch.bfloat16, H.device)
+    if bias is None or "db" not in need:
+        db = None
+    elif db is None:
+        db = torch.empty(V, device=H.device, dtype=torch.float32)
+    else:
+        assert db.device == H.device and db.dtype == torch.float32 and db.is_contiguous() and db.numel() == V
+    return dH, dW, db
+
+
+def _grad_args(t):
+    return (None, L.DGX_BF16, 0) if t is None else (t.data_ptr(), _DT[t.dtype], _pitch(t))
+
+
+def linear_distill_fwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,
+                       bias: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                       loss: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                       mean: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
+    """Distillation loss T^2 KL(softmax(teacher / T) || softmax((H W^T + bias) / T))
+    against a teacher's K largest logits per row: idx [R, K] int32 vocabulary
+    ids (outside [0, V): absent), teacher [R, K] fp32. Returns (loss [R],
+    lse [R]) with lse the log-sum-exp of the student's logits / T."""
+    R, V, d = _head_check(H, W, bias, idx, (teacher, loss, lse))
+    assert idx.dim() == 2 and teacher.shape == idx.shape
+    if loss is None:
+        loss = torch.empty(R, device=H.device, dtype=torch.float32)
+    if lse is None:
+        lse = torch.empty(R, device=H.device, dtype=torch.float32)
+    ws, wsb = _ws(workspace)
+    L.call("dgx_linear_distill_fwd", H.data_ptr(), _pitch(H), W.data_ptr(), _pitch(W), _ptr(bias), idx.data_ptr(),
+           teacher.data_ptr(), idx.shape[1], float(temperature), R, V, d, loss.data_ptr(), lse.data_ptr(), _ptr(mean),
+           ws, wsb, _stream(H))
+    return loss, lse
+
+
+def linear_distill_bwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, lse: torch.Tensor,
+                       *, bias: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                       dloss: Optional[torch.Tensor] = None, scale: float = 1.0, dH: Optional[torch.Tensor] = None,
+                       dW: Optional[torch.Tensor] = None, db: Optional[torch.Tensor] = None,
+                       need=("dH", "dW", "db"), accumulate: bool = False, workspace: Optional[torch.Tensor] = None):
+    """Gradients of sum_r scale * dloss[r] * loss[r]; arguments and results as linear_nll_bwd."""
+    R, V, d = _head_check(H, W, bias, idx, (teacher, lse, dloss))
+    assert idx.dim() == 2 and teacher.shape == idx.shape
+    dH, dW, db = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate)
+    ws, wsb = _ws(workspace)
+    L.call("dgx_linear_distill_bwd", H.data_ptr(), _pitch(H), W.data_ptr(), _pitch(W), _ptr(bias), idx.data_ptr(),
+           teacher.data_ptr(), idx.shape[1], float(temperature), lse.data_ptr(), _ptr(dloss), float(scale), R, V, d,
+           *_grad_args(dH), *_grad_args(dW), _ptr(db), int(accumulate), ws, wsb, _stream(H))
+    return dH, dW, db
+
+
+def _row_ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def embed_fwd(tok: torch.Tensor, W: torch.Tensor, *, scale: float = 1.0, pos: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x[i] = scale * W[tok[i]] (+ pos[i % len(pos)]): tok int32 of any shape
+    (taken flat), W [V, d] fp32 or bf16, pos [S, d] fp32, out [n, d] fp32 or
+    bf16 (W's type by default). An id outside [0, V) gives a zero row (+ pos)."""
+    assert W.is_cuda and W.dtype in (torch.float32, torch.bfloat16) and W.dim() == 2 and W.stride(1) == 1
+    assert tok.device == W.device and tok.dtype == torch.int32 and tok.is_contiguous()
+    n, (V, d) = tok.numel(), W.shape
+    if pos is not None:
+        assert pos.device == W.device and pos.dtype == torch.float32 and pos.is_contiguous() and pos.dim() == 2 and pos.shape[1] == d
+    if out is None:
+        out = torch.empty(n, d, device=W.device, dtype=out_dtype or W.dtype)
+    assert out.device == W.device and out.shape == (n, d) and out.stride(1) == 1 and out.dtype in (torch.float32, torch.bfloat16)
+    L.call("dgx_embed_fwd", tok.data_ptr(), W.data_ptr(), _DT[W.dtype], _row_ld(W), _ptr(pos),
+           0 if pos is None else pos.shape[0], float(scale), out.data_ptr(), _DT[out.dtype], _row_ld(out), n, d, V,
+           _stream(W))
+    return out
+
+
+def embed_bwd_workspace_size(n: int, d: int, V: int) -> int:
+    return L.load().dgx_embed_bwd_workspace_size(n, d, V)
+
+
+def embed_bwd(tok: torch.Tensor, dx: torch.Tensor, V: int, *, scale: float = 1.0, out: Optional[torch.Tensor] = None,
+              out_dtype: torch.dtype = torch.float32, accumulate: bool = False,
+              workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dW[t] = scale * sum of dx[i] over tok[i] == t, in ascending i: dx [n, d]
+    fp32 or bf16, dW [V, d] of out_dtype (or the given `out`; accumulate adds
+    to an fp32 one). The same bits on every run."""
+    assert dx.is_cuda and dx.dtype in (torch.float32, torch.bfloat16) and dx.dim() == 2 and dx.stride(1) == 1
+    assert tok.device == dx.device and tok.dtype == torch.int32 and tok.is_contiguous() and tok.numel() == dx.shape[0]
+    n, d = dx.shape
+    if out is None:
+        assert not accumulate, "accumulate needs the tensor to add to"
+        out = torch.empty(V, d, device=dx.device, dtype=out_dtype)
+    assert out.device == dx.device and out.shape == (V, d) and out.stride(1) == 1 and out.dtype in (torch.float32, torch.bfloat16)
+    ws, wsb = _ws(workspace)
+    L.call("dgx_embed_bwd", tok.data_ptr(), dx.data_ptr(), _DT[dx.dtype], _row_ld(dx), float(scale), out.data_ptr(),
+           _DT[out.dtype], _row_ld(out), n, d, V, int(accumulate), ws, wsb, _stream(dx))
+    return out
+
+
 def tp_shard(N: int, world: int, rank: int):
     col0, ncol = C.c_int(0), C.c_int(0)
     L.load().dgx_tp_shard(N, world, rank, C.byref(col0), C.byref(ncol))

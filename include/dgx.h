@@ -387,6 +387,87 @@ dgx_status dgx_rows_to_heads(const void* src, int src_type, int ld, int col0, vo
 dgx_status dgx_heads_to_rows(const void* src, void* dst, int ld, int col0, int B, int S, int H, int D, void* stream);
 
 /*
+ * Vocabulary head: linear layer, softmax and loss of a language model in one
+ * operator, in pieces of the vocabulary. The logits
+ *   z_rj = (H_r . W_j + bias_j) / T        (T = 1 for the hard target)
+ * of R rows over V columns are never kept: the forward leaves the loss and the
+ * log-sum-exp of each row, the backward recomputes a piece of z at a time.
+ *   H    [R][ldh] bf16, W [V][ldw] bf16 (the dream_linear weight layout),
+ *        16-byte aligned, pitches multiples of 8 elements and >= d
+ *   bias [V] fp32 or NULL (-inf or the lowest float masks a column)
+ *   products bf16 with fp32 accumulation; softmax, losses and sums fp32.
+ * Forward: loss [R] and lse [R] (log-sum-exp of z), fp32; mean (NULL, or one
+ * float) receives sum(loss) / R.
+ * Backward: with w_r = dloss[r] (dloss NULL: 1), 0 for a row without a target,
+ *   G_rj = scale * w_r * dloss_r/dz_rj / T
+ *   dH = G W   [R][lddh]   dW = G^T H   [V][lddw]   db = sum_r G   [V] fp32
+ * each of them skipped when NULL; dH and dW DGX_F32 or DGX_BF16 with 16-byte
+ * aligned rows. softmax - target is rounded to bf16 as the operand of the two
+ * products (scale is applied after them, in fp32); db is summed unrounded.
+ * accumulate = 1 adds to dW (fp32) and db. Every result is the same bits on
+ * every run. workspace: dgx_linear_*_workspace_size() bytes, 128-byte aligned,
+ * or NULL for the library's own buffer; its contents need not survive between
+ * calls. Rows of H must be finite even where the row has no target (0 * inf in
+ * dW); a row without a target has loss 0 and dH 0.
+ *
+ * dgx_linear_nll_*: loss_r = lse_r - z_{r,target[r]}; a target outside [0, V)
+ * means the row has none.
+ * Joins dream_linear, log_softmax and nll_loss (runtime/ops/elementwise.inc:
+ * 1432-1603) and their backward (runtime/ops/autograd.inc:156-245).
+ */
+dgx_status dgx_linear_nll_fwd(const void* H, int ldh, const void* W, int ldw, const float* bias, const int* target,
+                              int R, int V, int d, float* loss, float* lse, float* mean, void* workspace,
+                              size_t workspace_bytes, void* stream);
+dgx_status dgx_linear_nll_bwd(const void* H, int ldh, const void* W, int ldw, const float* bias, const int* target,
+                              const float* lse, const float* dloss, float scale, int R, int V, int d, void* dH,
+                              dgx_dtype dh_type, int lddh, void* dW, dgx_dtype dw_type, int lddw, float* db,
+                              int accumulate, void* workspace, size_t workspace_bytes, void* stream);
+size_t dgx_linear_nll_workspace_size(int R, int V, int d, int backward);
+/*
+ * dgx_linear_distill_*: distillation from a teacher's K largest logits per
+ * row, 1 <= K <= 256: idx [R][K] vocabulary ids (one outside [0, V) is an
+ * absent entry), teacher [R][K] fp32 logits, temperature T > 0:
+ *   q_r = softmax of teacher_r / T over the row's present entries
+ *   loss_r = T^2 * sum_k q_rk (log q_rk - z_{r,idx_rk} + lse_r)
+ * A row whose entries are all absent (or -inf) has no target. An id that
+ * repeats in a row counts with the sum of its probabilities. The reference
+ * has no counterpart; the student's head is dream_linear + log_softmax.
+ */
+dgx_status dgx_linear_distill_fwd(const void* H, int ldh, const void* W, int ldw, const float* bias, const int* idx,
+                                  const float* teacher, int K, float temperature, int R, int V, int d, float* loss,
+                                  float* lse, float* mean, void* workspace, size_t workspace_bytes, void* stream);
+dgx_status dgx_linear_distill_bwd(const void* H, int ldh, const void* W, int ldw, const float* bias, const int* idx,
+                                  const float* teacher, int K, float temperature, const float* lse,
+                                  const float* dloss, float scale, int R, int V, int d, void* dH, dgx_dtype dh_type,
+                                  int lddh, void* dW, dgx_dtype dw_type, int lddw, float* db, int accumulate,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+size_t dgx_linear_distill_workspace_size(int R, int V, int d, int K, int backward);
+
+/*
+ * Token embedding with a scale: x_i = scale * W[tok_i] (+ P[i % S]), a token
+ * id outside [0, V) gives a zero row (plus P). W [V][ldw] and x [n][ldx] are
+ * DGX_F32 or DGX_BF16 each, P [S][d] fp32 or NULL; any d, pitch and alignment.
+ * Extends dgx_embedding_fwd (dream_embedding, runtime/nn/training.inc:579-600)
+ * by the scale, the types and the pitches.
+ */
+dgx_status dgx_embed_fwd(const int* tok, const void* W, dgx_dtype w_type, int ldw, const float* P, int S, float scale,
+                         void* x, dgx_dtype x_type, int ldx, int n, int d, int V, void* stream);
+/*
+ * The table's gradient, dW_t (+)= scale * sum over i with tok_i = t of dx_i:
+ * fp32 sums in ascending i (within fixed groups of i where a token repeats
+ * often), rounded once, the same bits on every run. accumulate = 0 writes
+ * every row of dW (zero where the token does not occur); accumulate = 1 (fp32
+ * dW) adds to the rows of the tokens that occur and leaves the others alone.
+ * workspace: dgx_embed_bwd_workspace_size() bytes, 16-byte aligned, or NULL
+ * for the library's own buffer.
+ * dgx_embedding_bwd (runtime/ops/autograd.inc:330-341) adds with fp32 atomics.
+ */
+dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int lddx, float scale, void* dW,
+                         dgx_dtype dw_type, int lddw, int n, int d, int V, int accumulate, void* workspace,
+                         size_t workspace_bytes, void* stream);
+size_t dgx_embed_bwd_workspace_size(int n, int d, int V);
+
+/*
  * Column-parallel tensor-parallel GEMM over `world` GPUs, one process per GPU.
  * Each rank holds all of A [M,K] and its column shard of B ([K, n_r] with the
  * reference's widths: base = N/world, the first N%world shards one wider).

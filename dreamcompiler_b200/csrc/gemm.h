@@ -57,6 +57,10 @@ inline bool extras_tma_aligned(const GemmArgs& a) {
   return true;
 }
 
+// 128-byte-swizzled 2-D bf16 tensor map [outer][inner] with `pitch_bytes` rows.
+bool encode_2d_bf16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch_bytes,
+                    uint32_t box_inner, uint32_t box_outer);
+
 // 2-SM bf16 kernel (gemm2.cu) and the algorithm switch.
 bool gemm2_eligible(const GemmArgs& a, const void* A, const void* B);
 cudaError_t gemm2_launch(const GemmArgs& args, const void* A, const void* B, cudaStream_t stream);

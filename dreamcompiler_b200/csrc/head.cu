@@ -43,8 +43,8 @@ __device__ __forceinline__ float warp_max(float v) {
 // entries before it (K <= 256: at most 8 x 256 comparisons per lane).
 __global__ void head_lists_kernel(const int* __restrict__ idx, const float* __restrict__ teacher, int R, int V, int K,
                                   float inv_t, int* __restrict__ sid, float* __restrict__ sq,
-                                  float* __restrict__ live) {
-  __shared__ int ids_s[4][kHeadMaxK];
+                                  float* __restrict__ live, uint16_t* __restrict__ start, int slots) {
+  __shared__ int ids_s[4][kHeadMaxK], sorted_s[4][kHeadMaxK];
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.x * 4 + w;
   if (row >= R) return;
@@ -74,53 +74,63 @@ __global__ void head_lists_kernel(const int* __restrict__ idx, const float* __re
     const float q = (any && id != kNoId) ? expf((tr[k] - mx) * inv_t) * inv_s : 0.f;
     sid[(size_t)row * K + rank] = id;
     sq[(size_t)row * K + rank] = q;
+    sorted_s[w][rank] = id;
   }
   if (lane == 0) live[row] = any ? 1.f : 0.f;
+  __syncwarp();
+  for (int t = lane; t < slots; t += 32) {
+    int lo = 0, hi = K;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sorted_s[w][mid] < t * 128)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    start[(size_t)row * slots + t] = (uint16_t)lo;
+  }
 }
 
 // ---------------------------------------------------------------- forward
-// Row statistics of one piece of logits z [R][ldz] (columns c0 .. c0 + n of
-// the vocabulary): (max, sum of exp((z - max) / T)) into part[row], and the
-// raw logits at the target's ids into zs. One warp per row.
-__global__ void head_stats_kernel(const float* __restrict__ z, int ldz, int c0, int n, int R, float inv_t,
-                                  const int* __restrict__ sid, int K, float* __restrict__ zs,
-                                  float2* __restrict__ part) {
-  const int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= R) return;
-  const float* zr = z + (size_t)row * ldz;
-  float mx = -INFINITY;
-  for (int j = lane; j < n; j += 32) mx = fmaxf(mx, zr[j]);
-  mx = warp_max(mx);
-  const float base = mx == -INFINITY ? 0.f : mx;
-  float s = 0.f;
-  for (int j = lane; j < n; j += 32) s += expf((zr[j] - base) * inv_t);
-  s = warp_sum(s);
-  if (lane == 0) part[row] = make_float2(mx, s);
-  for (int k = lane; k < K; k += 32) {
-    const int id = sid[(size_t)row * K + k];
-    if (id >= c0 && id < c0 + n) zs[(size_t)row * K + k] = zr[id - c0];
-  }
-}
-
-// lse and loss from the partial statistics part[t][R] of `nt` pieces. One warp
-// per row. Hard target: sq == null.
-__global__ void head_finish_kernel(const float2* __restrict__ part, int nt, int R, int V, float t, float inv_t,
-                                   const int* __restrict__ sid, const float* __restrict__ sq, int K,
-                                   const float* __restrict__ zs, float* __restrict__ loss, float* __restrict__ lse) {
-  const int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= R) return;
-  float m = -INFINITY, s = 0.f;
-  for (int i = lane; i < nt; i += 32) {
-    const float2 p = part[(size_t)i * R + row];
-    const float mn = fmaxf(m, p.x), base = mn == -INFINITY ? 0.f : mn;
-    s = s * expf((m - base) * inv_t) + p.y * expf((p.x - base) * inv_t);
+// lse and loss from the statistics part[slot][R] (max of the raw logits and
+// sum of exp((z - max) / T) over 128 columns each). A block owns 32 rows, one
+// per lane; its 32 warps walk the slots and their results are joined through
+// shared memory in a fixed order. Hard target: sq == null.
+__global__ void __launch_bounds__(1024) head_finish_kernel(
+    const float2* __restrict__ part, int slots, int R, int V, float t, float inv_t, const int* __restrict__ sid,
+    const float* __restrict__ sq, int K, const float* __restrict__ zs, float* __restrict__ loss,
+    float* __restrict__ lse) {
+  __shared__ float2 ms[32][33];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row0 = blockIdx.x * 32;
+  auto join = [inv_t](float& m, float& s, float m2, float s2) {
+    const float mn = fmaxf(m, m2), base = mn == -INFINITY ? 0.f : mn;
+    s = s * expf((m - base) * inv_t) + s2 * expf((m2 - base) * inv_t);
     m = mn;
+  };
+  float m = -INFINITY, s = 0.f;
+  if (row0 + lane < R)
+    for (int i = w; i < slots; i += 32) {
+      const float2 p = part[(size_t)i * R + row0 + lane];
+      join(m, s, p.x, p.y);
+    }
+  ms[w][lane] = make_float2(m, s);
+  __syncthreads();
+  // warp w finishes row row0 + w: lane i holds warp i's part
+  const int row = row0 + w;
+  if (row >= R) return;
+  m = ms[lane][w].x;
+  s = ms[lane][w].y;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    join(m, s, m2, s2);
   }
-  const float mr = warp_max(m), base = mr == -INFINITY ? 0.f : mr;
-  s = warp_sum(s * expf((m - base) * inv_t));
-  const float log_s = logf(s);
-  // z - lse = (raw - max)/T - log s: the subtraction of the maximum first
-  // keeps the loss accurate when the logits are large
+  // lanes may differ in the last bit of s (the two sides add in either order)
+  s = __shfl_sync(0xffffffffu, s, 0);
+  const float base = m == -INFINITY ? 0.f : m, log_s = logf(s);
+  // z - lse = (raw - max)/T - log s: subtracting the maximum first keeps the
+  // loss accurate when the logits are large
   float l = 0.f;
   for (int k = lane; k < K; k += 32) {
     const int id = sid[(size_t)row * K + k];
@@ -154,40 +164,6 @@ __global__ void head_mean_kernel(const float* __restrict__ loss, int R, float* _
 // ---------------------------------------------------------------- backward
 constexpr int kSlabRows = 32;  // rows per partial column sum
 
-// G of one piece from its logits: a block owns kSlabRows rows and 256 columns,
-// one column per thread. G is rounded to bf16 (the operand of the gradient
-// GEMMs); the column sums are taken before the rounding.
-__global__ void head_grad_kernel(const float* __restrict__ z, int ldz, int c0, int n, int R, int V, float inv_t,
-                                 const float* __restrict__ lse, const float* __restrict__ dloss,
-                                 const float* __restrict__ live, const int* __restrict__ sid,
-                                 const float* __restrict__ sq, int K, __nv_bfloat16* __restrict__ g, int ldg,
-                                 float* __restrict__ dbp) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  const int r0 = blockIdx.y * kSlabRows, r1 = min(R, r0 + kSlabRows);
-  if (j >= ldg) return;
-  float col = 0.f;
-  for (int r = r0; r < r1; ++r) {
-    float w;
-    if (live) {
-      w = live[r];
-    } else {
-      const int t = sid[r];
-      w = (t >= 0 && t < V) ? 1.f : 0.f;
-    }
-    float v = 0.f;
-    if (w != 0.f && j < n) {
-      if (dloss) w = dloss[r];
-      v = expf(z[(size_t)r * ldz + j] * inv_t - lse[r]);
-      for (int k = 0; k < K; ++k)
-        if (sid[(size_t)r * K + k] == c0 + j) v -= sq ? sq[(size_t)r * K + k] : 1.f;
-      v *= w;
-    }
-    g[(size_t)r * ldg + j] = __float2bfloat16_rn(v);
-    col += v;
-  }
-  if (dbp && j < n) dbp[(size_t)blockIdx.y * n + j] = col;
-}
-
 // db[j] (+)= scale * sum over slabs of dbp[slab][j], in order.
 __global__ void head_db_kernel(const float* __restrict__ dbp, int slabs, int n, float scale, int accumulate,
                                float* __restrict__ db) {
@@ -215,31 +191,19 @@ __global__ void head_out_kernel(const float* __restrict__ acc, int rows, int d, 
   }
 }
 
-constexpr size_t kPieceBytes = 256u << 20;  // fp32 logits of one piece
+// Columns of one piece of the vocabulary in the backward: G (bf16, R rows) of
+// about 256 MB, so that its buffer stays far below the logits while the two
+// gradient products get a long enough piece to fill the GPU.
+constexpr size_t kPieceBytes = 256u << 20;
 
 size_t align128(size_t b) { return (b + 127) & ~size_t(127); }
 
-// Columns of one piece: as many as keep R x columns fp32 logits within
-// kPieceBytes, a multiple of 256.
 int piece_cols(int R, int V) {
-  const long long c = (long long)(kPieceBytes / 4 / (size_t)R) / 256 * 256;
-  return (int)std::min<long long>(std::max<long long>(c, 256), (V + 255) / 256 * 256);
+  const long long c = (long long)(kPieceBytes / 2 / (size_t)R) / 256 * 256;
+  return (int)std::min<long long>(std::max<long long>(c, 256), ((long long)V + 255) / 256 * 256);
 }
 
-dgx_status piece_logits(const HeadArgs& a, int c0, int n, float* z, int ldz, cudaStream_t s) {
-  GemmArgs g{};
-  g.M = a.R;
-  g.N = n;
-  g.K = a.d;
-  g.lda = a.ldh;
-  g.ldb = a.ldw;
-  g.ldc = ldz;
-  g.transB = 1;
-  g.C = z;
-  g.bias = a.bias ? a.bias + c0 : nullptr;
-  g.err = a.err;
-  return gemm_run(g, a.H, (const __nv_bfloat16*)a.W + (size_t)c0 * a.ldw, DGX_BF16, 0, nullptr, 0, s);
-}
+int num_slots(int V) { return (int)(((long long)V + 255) / 256 * 2); }
 
 struct Carve {
   char* p;
@@ -251,47 +215,66 @@ struct Carve {
   }
 };
 
+size_t list_bytes(int R, int V, int K) {
+  return 2 * align128((size_t)R * K * 4) + align128((size_t)R * 4) + align128((size_t)R * num_slots(V) * 2);
+}
+
+// Sorted target lists of the soft target (the hard one is its own list).
+void target_lists(const HeadArgs& a, Carve& c, HeadTcArgs& t, cudaStream_t s) {
+  t.sid = a.idx;
+  t.K = a.K;
+  if (!a.teacher) return;
+  int* si = c.take<int>((size_t)a.R * a.K);
+  float* q = c.take<float>((size_t)a.R * a.K);
+  float* live = c.take<float>(a.R);
+  t.slots = num_slots(a.V);
+  uint16_t* start = c.take<uint16_t>((size_t)a.R * t.slots);
+  head_lists_kernel<<<(a.R + 3) / 4, 128, 0, s>>>(a.idx, a.teacher, a.R, a.V, a.K, a.inv_t, si, q, live, start,
+                                                  t.slots);
+  t.sid = si;
+  t.sq = q;
+  t.live = live;
+  t.start = start;
+}
+
+HeadTcArgs tc_args(const HeadArgs& a) {
+  HeadTcArgs t{};
+  t.R = a.R;
+  t.V = a.V;
+  t.d = a.d;
+  t.inv_t = a.inv_t;
+  t.k = a.inv_t * 1.4426950408889634f;
+  t.bias = a.bias;
+  t.err = a.err;
+  return t;
+}
+
 }  // namespace
 
 size_t head_fwd_scratch_bytes(int R, int V, int d, int K, bool lists) {
-  const int pc = piece_cols(R, V), nt = (V + pc - 1) / pc;
-  size_t b = align128((size_t)R * pc * 4) + align128((size_t)nt * R * 8) + align128((size_t)R * K * 4);
-  if (lists) b += 2 * align128((size_t)R * K * 4) + align128((size_t)R * 4);
-  return b;
+  (void)d;
+  const int slots = (V + 127) / 128;
+  return align128((size_t)slots * R * 8) + align128((size_t)R * K * 4) + (lists ? list_bytes(R, V, K) : 0);
 }
 
 size_t head_bwd_scratch_bytes(int R, int V, int d, int K, bool lists) {
   const int pc = piece_cols(R, V);
-  size_t b = align128((size_t)R * pc * 4) + align128((size_t)R * pc * 2) +
-             align128((size_t)((R + kSlabRows - 1) / kSlabRows) * pc * 4) + align128((size_t)R * d * 4) +
-             align128((size_t)pc * d * 4);
-  if (lists) b += 2 * align128((size_t)R * K * 4) + align128((size_t)R * 4);
-  return b;
+  return align128((size_t)R * pc * 2) + align128((size_t)((R + kSlabRows - 1) / kSlabRows) * pc * 4) +
+         align128((size_t)R * d * 4) + align128((size_t)pc * d * 4) + (lists ? list_bytes(R, V, K) : 0);
 }
 
 dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s) {
-  const int pc = piece_cols(a.R, a.V), nt = (a.V + pc - 1) / pc;
+  const int slots = (a.V + 127) / 128;
   Carve c{(char*)ws};
-  float* z = c.take<float>((size_t)a.R * pc);
-  float2* part = c.take<float2>((size_t)nt * a.R);
-  float* zs = c.take<float>((size_t)a.R * a.K);
-  const int* sid = a.idx;
-  const float* sq = nullptr;
-  if (a.teacher) {
-    int* si = c.take<int>((size_t)a.R * a.K);
-    float* q = c.take<float>((size_t)a.R * a.K);
-    float* live = c.take<float>(a.R);
-    head_lists_kernel<<<(a.R + 3) / 4, 128, 0, s>>>(a.idx, a.teacher, a.R, a.V, a.K, a.inv_t, si, q, live);
-    sid = si;
-    sq = q;
-  }
-  for (int t = 0; t < nt; ++t) {
-    const int c0 = t * pc, n = std::min(pc, a.V - c0);
-    const dgx_status st = piece_logits(a, c0, n, z, pc, s);
-    if (st != DGX_OK) return st;
-    head_stats_kernel<<<(a.R + 7) / 8, 256, 0, s>>>(z, pc, c0, n, a.R, a.inv_t, sid, a.K, zs, part + (size_t)t * a.R);
-  }
-  head_finish_kernel<<<(a.R + 7) / 8, 256, 0, s>>>(part, nt, a.R, a.V, a.t, a.inv_t, sid, sq, a.K, zs, a.loss, a.lse);
+  HeadTcArgs t = tc_args(a);
+  t.part = c.take<float2>((size_t)slots * a.R);
+  t.zs = c.take<float>((size_t)a.R * a.K);
+  t.n = a.V;
+  target_lists(a, c, t, s);
+  const cudaError_t e = head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, false, nullptr, 0, s);
+  if (e != cudaSuccess) return cuda_status(e, "head forward");
+  head_finish_kernel<<<(a.R + 31) / 32, 1024, 0, s>>>(t.part, slots, a.R, a.V, a.t, a.inv_t, t.sid, t.sq, a.K, t.zs,
+                                                      a.loss, a.lse);
   if (a.mean) head_mean_kernel<<<1, 1024, 0, s>>>(a.loss, a.R, a.mean);
   return cuda_status(cudaGetLastError(), "head forward");
 }
@@ -299,30 +282,24 @@ dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s) {
 dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
   const int pc = piece_cols(a.R, a.V), slabs = (a.R + kSlabRows - 1) / kSlabRows;
   Carve c{(char*)ws};
-  float* z = c.take<float>((size_t)a.R * pc);
+  HeadTcArgs t = tc_args(a);
   __nv_bfloat16* g = c.take<__nv_bfloat16>((size_t)a.R * pc);
   float* dbp = c.take<float>((size_t)slabs * pc);
   float* dh = c.take<float>((size_t)a.R * a.d);
   float* dw = c.take<float>((size_t)pc * a.d);
-  const int* sid = a.idx;
-  const float *sq = nullptr, *live = nullptr;
-  if (a.teacher) {
-    int* si = c.take<int>((size_t)a.R * a.K);
-    float* q = c.take<float>((size_t)a.R * a.K);
-    float* lv = c.take<float>(a.R);
-    head_lists_kernel<<<(a.R + 3) / 4, 128, 0, s>>>(a.idx, a.teacher, a.R, a.V, a.K, a.inv_t, si, q, lv);
-    sid = si;
-    sq = q;
-    live = lv;
-  }
+  target_lists(a, c, t, s);
+  t.dbp = a.db ? dbp : nullptr;
+  t.dloss = a.dloss;
+  t.lse = a.lse;
   const int grid_out = num_sms() * 8;
   for (int c0 = 0; c0 < a.V; c0 += pc) {
     const int n = std::min(pc, a.V - c0);
-    dgx_status st = piece_logits(a, c0, n, z, pc, s);
-    if (st != DGX_OK) return st;
-    head_grad_kernel<<<dim3(pc / 256, slabs), 256, 0, s>>>(z, pc, c0, n, a.R, a.V, a.inv_t, a.lse, a.dloss, live, sid,
-                                                           sq, a.K, g, pc, a.db ? dbp : nullptr);
+    t.c0 = c0;
+    t.n = n;
+    const cudaError_t e = head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, true, g, pc, s);
+    if (e != cudaSuccess) return cuda_status(e, "head backward");
     if (a.db) head_db_kernel<<<(n + 255) / 256, 256, 0, s>>>(dbp, slabs, n, a.scale, a.accumulate, a.db + c0);
+    dgx_status st = DGX_OK;
     if (a.dH) {  // dh += G W
       GemmArgs m{};
       m.M = a.R;

@@ -9,7 +9,8 @@
 
 namespace dgx {
 
-constexpr int kHeadMaxK = 256;  // teacher entries per row
+constexpr int kHeadMaxK = 256;          // teacher entries per row
+constexpr int kHeadMaxRows = 1 << 23;   // rows, and columns of the vocabulary: tile counts fit 32 bits
 
 // One problem: logits z = (H . W^T + bias) / T of R rows over V columns, and a
 // sparse target per row: K ids with K probabilities. The hard target is K = 1
@@ -36,6 +37,28 @@ struct HeadArgs {
   int accumulate;      // dW (fp32) and db are added to
   uint32_t* err;
 };
+
+// One launch of the tensor-core logits kernel (head_tc.cu): columns
+// [c0, c0 + n) of the vocabulary, c0 a multiple of 256.
+struct HeadTcArgs {
+  int R, V, d, K, c0, n;
+  int tiles_m, tiles_n;     // filled by the launcher
+  float inv_t, k;           // 1 / T, log2(e) / T
+  const float* bias;        // [V] or null
+  const int* sid;           // [R][K] target ids, ascending when K > 1
+  const float* sq;          // [R][K] their probabilities, or null (1)
+  const uint16_t* start;    // [R][slots] first entry with id >= 128 * slot, or null (K = 1)
+  int slots;
+  float* zs;                // [R][K] out: raw logits at the ids (statistics)
+  float2* part;             // [ceil(n / 128)][R] out: (max, sum) per 128 columns (statistics)
+  const float* live;        // [R] 0 where the row has no target, or null (id in [0, V))
+  const float* dloss;       // [R] or null
+  const float* lse;         // [R]
+  float* dbp;               // [ceil(R / 32)][n] out: column sums per 32 rows, or null (gradient)
+  uint32_t* err;
+};
+cudaError_t head_logits_tc(HeadTcArgs a, const void* H, int ldh, const void* W, int ldw, bool grad, void* g, int ldg,
+                           cudaStream_t s);
 
 size_t head_fwd_scratch_bytes(int R, int V, int d, int K, bool lists);
 size_t head_bwd_scratch_bytes(int R, int V, int d, int K, bool lists);

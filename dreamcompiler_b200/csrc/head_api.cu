@@ -14,6 +14,8 @@ namespace {
 
 dgx_status head_check(const char* op, const void* H, int ldh, const void* W, int ldw, int R, int V, int d, int K) {
   if (R < 0 || V <= 0 || d <= 0) return set_error(DGX_EINVAL, "%s: bad size R=%d V=%d d=%d", op, R, V, d);
+  if (R > kHeadMaxRows || V > kHeadMaxRows)
+    return set_error(DGX_EINVAL, "%s: R=%d or V=%d above %d", op, R, V, kHeadMaxRows);
   if (K < 1 || K > kHeadMaxK) return set_error(DGX_EINVAL, "%s: K=%d (1..%d entries per row)", op, K, kHeadMaxK);
   if (ldh < d || ldw < d || ldh % 8 || ldw % 8)
     return set_error(DGX_EINVAL, "%s: row pitch ldh=%d ldw=%d (>= d=%d and a multiple of 8)", op, ldh, ldw, d);

@@ -1,0 +1,382 @@
+// Tensor-core kernels of the vocabulary head (head.cu drives them): the logits
+// of 256 rows x 256 columns of the vocabulary are one tcgen05 accumulator
+// tile over a CTA pair (cta_group::2, each SM its own 128 rows), consumed by
+// the epilogue where they stand. No logit is written to memory.
+//
+//   head_logits_kernel<kStats>   per row and 128 columns: max and sum of
+//                                exp((z - max) / T), and z at the target's ids
+//   head_logits_kernel<kGrad>    G = w (exp(z/T - lse) - q) as bf16, and its
+//                                column sums before the rounding
+//
+// Both run the main loop of gemm2_kernel (TMA operand ring, one MMA-issuing
+// thread in the leader, two TMEM accumulators) with eight epilogue warps, two
+// per TMEM lane quarter, each taking 128 of the tile's 256 columns.
+#include <algorithm>
+
+#include "gemm.h"
+#include "head.h"
+#include "pair.cuh"
+#include "sm100.cuh"
+
+namespace dgx {
+namespace {
+
+constexpr int HD_BM = 128;  // rows per CTA (256 per pair)
+constexpr int HD_BN = 256;  // vocabulary columns per tile (128 W rows loaded per CTA)
+constexpr int HD_BK = 64;   // one 128-byte swizzled row of bf16
+constexpr int HD_STAGE = 2 * HD_BM * HD_BK * 2;  // 16 KB of H and 16 KB of W
+constexpr int HD_STAGES = 6;
+constexpr int HD_EPI_WARPS = 8;
+constexpr int HD_THREADS = 64 + 32 * HD_EPI_WARPS;
+constexpr int HD_SMEM = HD_STAGES * HD_STAGE + HD_EPI_WARPS * 4096 + 1024 + 256;
+constexpr uint32_t HD_TMEM_COLS = 512;
+
+constexpr int kStats = 0, kGrad = 1;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// One row's sparse target inside one tile: the entries of its sorted list from
+// the first id of this warp's columns on.
+struct Target {
+  const int* ids;   // [K] ascending
+  const float* qs;  // [K], or null: every q is 1
+  int k, K, nid;    // next entry and its id (INT_MAX: none)
+  __device__ __forceinline__ void next() {
+    ++k;
+    nid = k < K ? ids[k] : 0x7fffffff;
+  }
+};
+
+template <int MODE>
+__global__ void __launch_bounds__(HD_THREADS, 1)
+    head_logits_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW,
+                       const __grid_constant__ CUtensorMap tmG, HeadTcArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* out_stage = smem + HD_STAGES * HD_STAGE;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_stage + HD_EPI_WARPS * 4096);
+  uint64_t* empty_bar = full_bar + HD_STAGES;
+  uint64_t* accf_bar = empty_bar + HD_STAGES;  // [2]
+  uint64_t* acce_bar = accf_bar + 2;           // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acce_bar + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank_u32();
+  const bool leader = rank == 0;
+  WaitCtx wc{abort_flag, a.err};
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < HD_STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accf_bar[b], 1);
+      mbar_init(&acce_bar[b], 2 * HD_EPI_WARPS);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmH);
+    tma_prefetch_desc(&tmW);
+    if (MODE == kGrad) tma_prefetch_desc(&tmG);
+  }
+  if (warp == 1) {  // same warp in both CTAs, same destination offset
+    tmem_alloc2(tmem_slot, HD_TMEM_COLS);
+    tmem_relinquish2();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all2();  // both CTAs' barriers are initialised before any cross-CTA traffic
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int num_tiles = a.tiles_m * a.tiles_n;
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const int nk = (a.d + HD_BK - 1) / HD_BK;
+  // Tiles in groups of kGroup row tiles, row tiles innermost: the pairs that
+  // run together share a few W tiles and a few H tiles in L2.
+  constexpr int kGroup = 8;
+  auto coords = [&](int t, int& tm, int& tn) {
+    const int per_group = kGroup * a.tiles_n;
+    const int g = t / per_group, r = t - g * per_group;
+    const int gsize = min(a.tiles_m - g * kGroup, kGroup);
+    tm = g * kGroup + r % gsize;
+    tn = r / gsize;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs)
+    if (elect_one_lane()) {
+      uint32_t fill = 0;
+      for (int t = pair; t < num_tiles && !*abort_flag; t += npairs) {
+        int tm, tn;
+        coords(t, tm, tn);
+        const int m0 = tm * 2 * HD_BM + (int)rank * HD_BM;        // this CTA's 128 rows of H
+        const int n0 = tn * HD_BN + (int)rank * (HD_BN / 2);      // this CTA's 128 rows of W
+        for (int kb = 0; kb < nk; ++kb, ++fill) {
+          const int s = fill % HD_STAGES;
+          if (!mbar_wait(&empty_bar[s], ((fill / HD_STAGES) & 1) ^ 1, wc)) break;
+          uint8_t* sa = smem + s * HD_STAGE;
+          if (leader) mbar_arrive_expect_tx(&full_bar[s], 2 * HD_STAGE);
+          tma_load_2d_pair(sa, &tmH, &full_bar[s], kb * HD_BK, m0);
+          tma_load_2d_pair(sa + HD_STAGE / 2, &tmW, &full_bar[s], kb * HD_BK, n0);
+        }
+        if (*abort_flag) break;
+      }
+      // This CTA's copies have landed once the MMAs that read them are done.
+      const uint32_t first = fill > (uint32_t)HD_STAGES ? fill - HD_STAGES : 0;
+      for (uint32_t f = first; f < fill; ++f) mbar_drain(&empty_bar[f % HD_STAGES], (f / HD_STAGES) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader only)
+    if (leader && elect_one_lane()) {
+      constexpr uint32_t idesc = make_idesc(1, 0, 0, 2 * HD_BM, HD_BN);
+      uint32_t fill = 0, use = 0;
+      for (int t = pair; t < num_tiles; t += npairs, ++use) {
+        const int buf = use & 1;
+        if (!mbar_wait(&acce_bar[buf], ((use >> 1) & 1) ^ 1, wc)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + buf * HD_BN;
+        bool ok = true;
+        for (int kb = 0; kb < nk; ++kb, ++fill) {
+          const int s = fill % HD_STAGES;
+          if (!mbar_wait(&full_bar[s], (fill / HD_STAGES) & 1, wc)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * HD_STAGE), sb = sa + HD_STAGE / 2;
+#pragma unroll
+          for (int kk = 0; kk < HD_BK / 16; ++kk)
+            mma2_f16_ss(d_tmem, sw128_desc(sa + kk * 32, 16, 1024), sw128_desc(sb + kk * 32, 16, 1024), idesc,
+                        (kb > 0 || kk > 0) ? 1u : 0u);
+          tc_commit2_mc(&empty_bar[s], 0x3);
+        }
+        if (!ok) break;
+        tc_commit2_mc(&accf_bar[buf], 0x3);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
+    const int q = warp & 3;              // TMEM lane quarter this warp may access
+    const int half = (warp - 2) >> 2;    // its 128 columns of the tile
+    uint8_t* st = out_stage + (warp - 2) * 4096;
+    uint32_t issued = 0, use = 0;
+    for (int t = pair; t < num_tiles; t += npairs, ++use) {
+      const int buf = use & 1;
+      int tm, tn;
+      coords(t, tm, tn);
+      const int row0 = tm * 2 * HD_BM + (int)rank * HD_BM + q * 32, row = row0 + lane;
+      const int nbase = tn * HD_BN + half * 128;  // first column of this warp, within the piece
+      const bool row_ok = row < a.R;
+      // the row's target entries from this warp's columns on
+      Target tg{nullptr, nullptr, 0, 0, 0x7fffffff};
+      float w = 1.f, lse = 0.f;
+      if (row_ok) {
+        tg.ids = a.sid + (size_t)row * a.K;
+        tg.qs = a.sq ? a.sq + (size_t)row * a.K : nullptr;
+        tg.K = a.K;
+        tg.k = (a.start ? a.start[(size_t)row * a.slots + (a.c0 + nbase) / 128] : 0) - 1;
+        tg.next();
+        if (MODE == kGrad) {
+          const bool live = a.live ? a.live[row] != 0.f : (tg.nid >= 0 && tg.nid < a.V);
+          w = live ? (a.dloss ? a.dloss[row] : 1.f) : 0.f;
+          lse = a.lse[row];
+        }
+      } else if (MODE == kGrad) {
+        w = 0.f;
+      }
+      prefetch_bias_l1(a.bias, a.c0 + nbase, 128, a.V, lane);
+      if (!mbar_wait(&accf_bar[buf], (use >> 1) & 1, wc)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + buf * HD_BN + half * 128;
+      float m = -INFINITY, s = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 32) {
+        uint32_t r[32];
+        tmem_ld32(taddr + c, r);
+        const int n0 = nbase + c;          // column within the piece
+        const int j0 = a.c0 + n0;          // vocabulary id of column 0 of this chunk
+        float z[32];
+        if (a.bias) {
+#pragma unroll
+          for (int j8 = 0; j8 < 32; j8 += 8) {
+            float b8[8];
+            load_bias8(a.bias, j0 + j8, a.V, b8);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[j8 + i] = b8[i];
+          }
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[j] += __uint_as_float(r[j]);
+        } else {
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(r[j]);
+        }
+        if (c == 96) {  // this warp's last read of the accumulator
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (leader)
+              mbar_arrive(&acce_bar[buf]);
+            else
+              mbar_arrive_remote(&acce_bar[buf], 0);
+          }
+        }
+        if (n0 >= a.n) continue;  // uniform: nothing of the piece in this chunk
+        if constexpr (MODE == kStats) {
+          if (n0 + 32 > a.n) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (n0 + j >= a.n) z[j] = -INFINITY;
+          }
+          while (__any_sync(0xffffffffu, (unsigned)tg.nid - (unsigned)j0 < 32u)) {
+            const int at = (int)((unsigned)tg.nid - (unsigned)j0);
+            float v = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v = at == j ? z[j] : v;
+            if ((unsigned)at < 32u) {
+              a.zs[(size_t)row * a.K + tg.k] = v;
+              tg.next();
+            }
+          }
+          float cm = max3f(z[0], z[1], z[2]);
+#pragma unroll
+          for (int j = 3; j < 31; j += 2) cm = max3f(cm, z[j], z[j + 1]);
+          cm = fmaxf(cm, z[31]);
+          const float mn = fmaxf(m, cm);
+          const float base = mn == -INFINITY ? 0.f : mn;
+          float2 s0 = make_float2(s * ex2((m - base) * a.k), 0.f), s1 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            // subtract before scaling: exact for equal logits of any size
+            const float2 x = fsubmul2(z[j], z[j + 1], base, base, a.k, a.k);
+            const float2 y = fsubmul2(z[j + 2], z[j + 3], base, base, a.k, a.k);
+            s0 = fadd2(s0, ex2(x.x), ex2(x.y));
+            s1 = fadd2(s1, ex2(y.x), ex2(y.y));
+          }
+          s = (s0.x + s0.y) + (s1.x + s1.y);
+          m = mn;
+        } else {
+          // G: a row without a target is exactly zero, whatever its logits hold
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float2 x = ffma2(z[j], z[j + 1], a.inv_t, -lse);
+            z[j] = ex2(x.x * kLog2e) * w;
+            z[j + 1] = ex2(x.y * kLog2e) * w;
+          }
+          if (w == 0.f) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[j] = 0.f;
+          }
+          while (__any_sync(0xffffffffu, (unsigned)tg.nid - (unsigned)j0 < 32u)) {
+            const int at = (int)((unsigned)tg.nid - (unsigned)j0);
+            const bool hit = (unsigned)at < 32u;
+            const float qw = hit ? (tg.qs ? tg.qs[tg.k] : 1.f) * w : 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[j] -= at == j ? qw : 0.f;
+            if (hit) tg.next();
+          }
+          const int hb = (c & 32) ? 4 : 0;  // 16-byte units of this half of the 64-column box
+          if (!(c & 32)) {
+            if (lane == 0 && issued) bulk_wait_read0();
+            __syncwarp();
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<uint4*>(st + lane * 128 + (((u + hb) ^ (lane & 7)) << 4)) =
+                make_uint4(pack_bf16x2(z[8 * u], z[8 * u + 1]), pack_bf16x2(z[8 * u + 2], z[8 * u + 3]),
+                           pack_bf16x2(z[8 * u + 4], z[8 * u + 5]), pack_bf16x2(z[8 * u + 6], z[8 * u + 7]));
+          if ((c & 32) || n0 + 32 >= a.n) {  // box complete (or its second half lies past the piece)
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmG, st, nbase + (c & 64), row0);
+              bulk_commit();
+            }
+            ++issued;
+          }
+          if (a.dbp) {
+            // Column sums over the warp's 32 rows: 32 x 32 values, each step
+            // exchanging half of what is left with the lane 16, 8, ... away;
+            // lane j ends with column j (31 shuffles instead of 160).
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+              const bool up = lane & o;
+#pragma unroll
+              for (int j = 0; j < o; ++j) {
+                const float mine = up ? z[j + o] : z[j], give = up ? z[j] : z[j + o];
+                z[j] = mine + __shfl_xor_sync(0xffffffffu, give, o);
+              }
+            }
+            if (row0 < a.R && n0 + lane < a.n) a.dbp[(size_t)(row0 >> 5) * a.n + n0 + lane] = z[0];
+          }
+        }
+      }
+      if (MODE == kStats && row_ok && nbase < a.n) a.part[(size_t)(tn * 2 + half) * a.R + row] = make_float2(m, s);
+    }
+    if (MODE == kGrad && lane == 0) bulk_wait0();
+  }
+
+  // Neither CTA leaves (or frees TMEM) while its pair may still use its
+  // shared memory or TMEM.
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all2();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc2(tmem_base, HD_TMEM_COLS);
+  }
+}
+
+template <typename K>
+cudaError_t launch_pairs(K kern, int pairs, cudaStream_t s, const CUtensorMap& h, const CUtensorMap& w,
+                         const CUtensorMap& g, const HeadTcArgs& a) {
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, HD_SMEM);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * pairs);
+  cfg.blockDim = dim3(HD_THREADS);
+  cfg.dynamicSmemBytes = HD_SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, h, w, g, a);
+}
+
+}  // namespace
+
+// Logits of the piece [c0, c0 + n) of the vocabulary: row statistics
+// (grad = false) or G (grad = true, into g with pitch ldg).
+cudaError_t head_logits_tc(HeadTcArgs a, const void* H, int ldh, const void* W, int ldw, bool grad, void* g, int ldg,
+                           cudaStream_t s) {
+  CUtensorMap mh{}, mw{}, mg{};
+  const __nv_bfloat16* wp = (const __nv_bfloat16*)W + (size_t)a.c0 * ldw;
+  if (!encode_2d_bf16(&mh, H, a.d, a.R, (uint64_t)ldh * 2, HD_BK, HD_BM)) return cudaErrorInvalidValue;
+  if (!encode_2d_bf16(&mw, wp, a.d, a.n, (uint64_t)ldw * 2, HD_BK, HD_BN / 2)) return cudaErrorInvalidValue;
+  mg = mh;
+  if (grad && !encode_2d_bf16(&mg, g, a.n, a.R, (uint64_t)ldg * 2, 64, 32)) return cudaErrorInvalidValue;
+  a.tiles_m = (a.R + 2 * HD_BM - 1) / (2 * HD_BM);
+  a.tiles_n = (a.n + HD_BN - 1) / HD_BN;
+  const int pairs = (int)std::min<long long>((long long)a.tiles_m * a.tiles_n, num_sms() / 2);
+  return grad ? launch_pairs(head_logits_kernel<kGrad>, pairs, s, mh, mw, mg, a)
+              : launch_pairs(head_logits_kernel<kStats>, pairs, s, mh, mw, mg, a);
+}
+
+}  // namespace dgx

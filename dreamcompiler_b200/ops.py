@@ -21,7 +21,8 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the raw handle of torch.cuda.current_stream(t.device), without building a Stream object per call
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def version() -> str:

@@ -174,19 +174,37 @@ __global__ void head_db_kernel(const float* __restrict__ dbp, int slabs, int n, 
   db[j] = (accumulate ? db[j] : 0.f) + scale * s;
 }
 
-// out[r][j] (+)= scale * acc[r][j], rounded once to bf16 where asked.
-__global__ void head_out_kernel(const float* __restrict__ acc, int rows, int d, float scale, int bf16_out,
-                                int accumulate, void* __restrict__ out, int ldo) {
-  const long long total = (long long)rows * d;
+// out[r][j] (+)= scale * sum over slices of acc[slice][r][j], in order, rounded
+// once to bf16 where asked; four columns per thread (pitches are multiples of
+// four elements).
+__global__ void head_out_kernel(const float* __restrict__ acc, int slices, int rows, int d, int lda, float scale,
+                                int bf16_out, int accumulate, void* __restrict__ out, int ldo) {
+  const int dq = (d + 3) >> 2;
+  const long long total = (long long)rows * dq;
+  const size_t slice = (size_t)rows * lda;
   for (long long e = blockIdx.x * (long long)blockDim.x + threadIdx.x; e < total;
        e += (long long)gridDim.x * blockDim.x) {
-    const long long r = e / d, j = e % d;
-    const float v = scale * acc[e];
+    const long long r = e / dq;
+    const int j = (int)(e - r * dq) * 4;
+    const float* p = acc + (size_t)r * lda + j;
+    float4 v = *reinterpret_cast<const float4*>(p);
+    for (int i = 1; i < slices; ++i) {
+      const float4 u = *reinterpret_cast<const float4*>(p + i * slice);
+      v.x += u.x;
+      v.y += u.y;
+      v.z += u.z;
+      v.w += u.w;
+    }
+    const float f[4] = {scale * v.x, scale * v.y, scale * v.z, scale * v.w};
     if (bf16_out) {
-      reinterpret_cast<__nv_bfloat16*>(out)[r * ldo + j] = __float2bfloat16_rn(v);
+      __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(out) + r * ldo + j;
+      if (j + 4 <= d)
+        *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+      else
+        for (int i = 0; j + i < d; ++i) o[i] = __float2bfloat16_rn(f[i]);
     } else {
       float* o = reinterpret_cast<float*>(out) + r * ldo + j;
-      *o = accumulate ? *o + v : v;
+      for (int i = 0; i < 4 && j + i < d; ++i) o[i] = accumulate ? o[i] + f[i] : f[i];
     }
   }
 }
@@ -257,10 +275,29 @@ size_t head_fwd_scratch_bytes(int R, int V, int d, int K, bool lists) {
   return align128((size_t)slots * R * 8) + align128((size_t)R * K * 4) + (lists ? list_bytes(R, V, K) : 0);
 }
 
+// How the backward of one problem is cut: columns per piece, the slices of the
+// gradient sums and the scratch they need. Sized for dH and dW both wanted.
+struct Plan {
+  int pc, pieces, slabs, dp;
+  GradSplits sp;
+  bool dh_scratch;  // dH goes through fp32 scratch (several pieces, or slices)
+};
+static Plan make_plan(int R, int V, int d) {
+  Plan p;
+  p.pc = piece_cols(R, V);
+  p.pieces = (V + p.pc - 1) / p.pc;
+  p.slabs = (R + kSlabRows - 1) / kSlabRows;
+  p.dp = (d + 3) / 4 * 4;
+  p.sp = head_grad_splits(R, std::min(p.pc, V), d, true, true);
+  p.dh_scratch = p.pieces > 1 || p.sp.dh > 1;
+  return p;
+}
+
 size_t head_bwd_scratch_bytes(int R, int V, int d, int K, bool lists) {
-  const int pc = piece_cols(R, V);
-  return align128((size_t)R * pc * 2) + align128((size_t)((R + kSlabRows - 1) / kSlabRows) * pc * 4) +
-         align128((size_t)R * d * 4) + align128((size_t)pc * d * 4) + (lists ? list_bytes(R, V, K) : 0);
+  const Plan p = make_plan(R, V, d);
+  return align128((size_t)R * p.pc * 2) + align128((size_t)p.slabs * p.pc * 4) +
+         align128(p.dh_scratch ? (size_t)p.sp.dh * R * p.dp * 4 : 0) +
+         align128(p.sp.dw > 1 ? (size_t)p.sp.dw * std::min(p.pc, V) * p.dp * 4 : 0) + (lists ? list_bytes(R, V, K) : 0);
 }
 
 dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s) {
@@ -280,58 +317,44 @@ dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s) {
 }
 
 dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
-  const int pc = piece_cols(a.R, a.V), slabs = (a.R + kSlabRows - 1) / kSlabRows;
+  const Plan p = make_plan(a.R, a.V, a.d);
   Carve c{(char*)ws};
   HeadTcArgs t = tc_args(a);
-  __nv_bfloat16* g = c.take<__nv_bfloat16>((size_t)a.R * pc);
-  float* dbp = c.take<float>((size_t)slabs * pc);
-  float* dh = c.take<float>((size_t)a.R * a.d);
-  float* dw = c.take<float>((size_t)pc * a.d);
+  __nv_bfloat16* g = c.take<__nv_bfloat16>((size_t)a.R * p.pc);
+  float* dbp = c.take<float>((size_t)p.slabs * p.pc);
+  float* dh = p.dh_scratch ? c.take<float>((size_t)p.sp.dh * a.R * p.dp) : nullptr;
+  float* dw = p.sp.dw > 1 ? c.take<float>((size_t)p.sp.dw * std::min(p.pc, a.V) * p.dp) : nullptr;
   target_lists(a, c, t, s);
   t.dbp = a.db ? dbp : nullptr;
   t.dloss = a.dloss;
   t.lse = a.lse;
   const int grid_out = num_sms() * 8;
-  for (int c0 = 0; c0 < a.V; c0 += pc) {
-    const int n = std::min(pc, a.V - c0);
+  for (int c0 = 0; c0 < a.V; c0 += p.pc) {
+    const int n = std::min(p.pc, a.V - c0);
     t.c0 = c0;
     t.n = n;
-    const cudaError_t e = head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, true, g, pc, s);
+    cudaError_t e = head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, true, g, p.pc, s);
     if (e != cudaSuccess) return cuda_status(e, "head backward");
-    if (a.db) head_db_kernel<<<(n + 255) / 256, 256, 0, s>>>(dbp, slabs, n, a.scale, a.accumulate, a.db + c0);
-    dgx_status st = DGX_OK;
-    if (a.dH) {  // dh += G W
-      GemmArgs m{};
-      m.M = a.R;
-      m.N = a.d;
-      m.K = n;
-      m.lda = pc;
-      m.ldb = a.ldw;
-      m.ldc = a.d;
-      m.C = dh;
-      m.beta = c0 ? 1.f : 0.f;
-      m.err = a.err;
-      st = gemm_run(m, g, (const __nv_bfloat16*)a.W + (size_t)c0 * a.ldw, DGX_BF16, 0, nullptr, 0, s);
-      if (st != DGX_OK) return st;
-    }
-    if (a.dW) {  // dw = G^T H
-      GemmArgs m{};
-      m.M = n;
-      m.N = a.d;
-      m.K = a.R;
-      m.lda = pc;
-      m.ldb = a.ldh;
-      m.ldc = a.d;
-      m.transA = 1;
-      m.C = dw;
-      m.err = a.err;
-      st = gemm_run(m, g, a.H, DGX_BF16, 0, nullptr, 0, s);
-      if (st != DGX_OK) return st;
-      void* out = (char*)a.dW + (size_t)c0 * a.lddw * (a.dw_bf16 ? 2 : 4);
-      head_out_kernel<<<grid_out, 256, 0, s>>>(dw, n, a.d, a.scale, a.dw_bf16, a.accumulate, out, a.lddw);
-    }
+    if (a.db) head_db_kernel<<<(n + 255) / 256, 256, 0, s>>>(dbp, p.slabs, n, a.scale, a.accumulate, a.db + c0);
+    HeadGradTc m{};
+    m.G = g;
+    m.ldg = p.pc;
+    m.W = (const __nv_bfloat16*)a.W + (size_t)c0 * a.ldw;
+    m.ldw = a.ldw;
+    m.H = a.H;
+    m.ldh = a.ldh;
+    m.R = a.R;
+    m.n = n;
+    m.d = a.d;
+    m.err = a.err;
+    void* dw_out = a.dW ? (char*)a.dW + (size_t)c0 * a.lddw * (a.dw_bf16 ? 2 : 4) : nullptr;
+    if (a.dH) m.out[0] = dh ? GradOut{dh, 0, c0 > 0, p.dp, p.sp.dh, 1.f} : GradOut{a.dH, a.dh_bf16, 0, a.lddh, 1, a.scale};
+    if (a.dW) m.out[1] = dw ? GradOut{dw, 0, 0, p.dp, p.sp.dw, 1.f} : GradOut{dw_out, a.dw_bf16, a.accumulate, a.lddw, 1, a.scale};
+    e = head_grads_tc(m, s);
+    if (e != cudaSuccess) return cuda_status(e, "head backward");
+    if (a.dW && dw) head_out_kernel<<<grid_out, 256, 0, s>>>(dw, p.sp.dw, n, a.d, p.dp, a.scale, a.dw_bf16, a.accumulate, dw_out, a.lddw);
   }
-  if (a.dH) head_out_kernel<<<grid_out, 256, 0, s>>>(dh, a.R, a.d, a.scale, a.dh_bf16, 0, a.dH, a.lddh);
+  if (a.dH && dh) head_out_kernel<<<grid_out, 256, 0, s>>>(dh, p.sp.dh, a.R, a.d, p.dp, a.scale, a.dh_bf16, 0, a.dH, a.lddh);
   return cuda_status(cudaGetLastError(), "head backward");
 }
 

@@ -60,6 +60,27 @@ struct HeadTcArgs {
 cudaError_t head_logits_tc(HeadTcArgs a, const void* H, int ldh, const void* W, int ldw, bool grad, void* g, int ldg,
                            cudaStream_t s);
 
+// Both gradient products of one piece (head_grads.cu). out[0] is dH [R][ld],
+// out[1] dW [n][ld]; with splits > 1 the output is fp32 partial sums
+// [splits][rows][ld]. ptr null: the product is skipped.
+constexpr int kMaxSplits = 32;
+struct GradOut {
+  void* ptr;
+  int bf16, add, ld, splits;
+  float alpha;
+};
+struct HeadGradTc {
+  const void *G, *W, *H;  // [R][ldg], [n][ldw], [R][ldh] bf16
+  int ldg, ldw, ldh, R, n, d;
+  GradOut out[2];
+  uint32_t* err;
+};
+struct GradSplits {
+  int dh, dw;
+};
+GradSplits head_grad_splits(int R, int n, int d, bool want_dh, bool want_dw);
+cudaError_t head_grads_tc(const HeadGradTc& g, cudaStream_t s);
+
 size_t head_fwd_scratch_bytes(int R, int V, int d, int K, bool lists);
 size_t head_bwd_scratch_bytes(int R, int V, int d, int K, bool lists);
 dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s);

@@ -12,6 +12,8 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "common.h"
 #include "sm100.cuh"
@@ -30,42 +32,51 @@ struct Lane8 {
   static __device__ __forceinline__ int col(int lane, int k) { return VEC ? lane * 8 + k : lane + 32 * k; }
 };
 
-__device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
-  a = __uint_as_float(w << 16);
-  b = __uint_as_float(w & 0xFFFF0000u);
-}
-
-template <bool VEC>
-__device__ __forceinline__ void load8(const float* p, int lane, int left, float (&v)[8]) {
-  if constexpr (VEC) {
-    if (lane * 8 < left) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p + lane * 8));
-      const float4 b = __ldg(reinterpret_cast<const float4*>(p + lane * 8 + 4));
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// A lane's 8 elements of a row as loaded (bf16 stays packed until it is used,
+// so that twice the rows fit in the same registers).
+template <typename T, bool VEC>
+struct Row8 {
+  static constexpr bool kPacked = VEC && sizeof(T) == 2;
+  static constexpr int kRegs = kPacked ? 4 : 8;
+  uint32_t r[kRegs];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int k = 0; k < kRegs; ++k) r[k] = 0;
+  }
+  // p: the lane's slab of the row, `left` columns wide
+  __device__ __forceinline__ void load(const T* p, int lane, int left) {
+    if constexpr (VEC) {
+      if (lane * 8 < left) {
+        const uint4* q = reinterpret_cast<const uint4*>(p + lane * 8);
+#pragma unroll
+        for (int k = 0; k < kRegs / 4; ++k) {
+          const uint4 a = __ldg(q + k);
+          r[4 * k] = a.x, r[4 * k + 1] = a.y, r[4 * k + 2] = a.z, r[4 * k + 3] = a.w;
+        }
+      } else {
+        zero();
+      }
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+      for (int k = 0; k < 8; ++k) {
+        float v = 0.f;
+        if (lane + 32 * k < left) {
+          if constexpr (sizeof(T) == 2)
+            v = __bfloat162float(p[lane + 32 * k]);
+          else
+            v = __ldg(p + lane + 32 * k);
+        }
+        r[k] = __float_as_uint(v);
+      }
     }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = lane + 32 * k < left ? __ldg(p + lane + 32 * k) : 0.f;
   }
-}
-template <bool VEC>
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, int lane, int left, float (&v)[8]) {
-  if constexpr (VEC) {
-    uint4 a = make_uint4(0, 0, 0, 0);
-    if (lane * 8 < left) a = __ldg(reinterpret_cast<const uint4*>(p + lane * 8));
-    unpack2(a.x, v[0], v[1]);
-    unpack2(a.y, v[2], v[3]);
-    unpack2(a.z, v[4], v[5]);
-    unpack2(a.w, v[6], v[7]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = lane + 32 * k < left ? __bfloat162float(p[lane + 32 * k]) : 0.f;
+  __device__ __forceinline__ float get(int k) const {
+    if constexpr (kPacked)
+      return __uint_as_float(k & 1 ? r[k >> 1] & 0xFFFF0000u : r[k >> 1] << 16);
+    else
+      return __uint_as_float(r[k]);
   }
-}
+};
 template <bool VEC>
 __device__ __forceinline__ void store8(float* p, int lane, int left, const float (&v)[8]) {
   if constexpr (VEC) {
@@ -95,111 +106,147 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, int lane, int left, con
 constexpr int kSlab = 256;  // columns per warp
 
 // ---------------------------------------------------------------- forward
-// One warp per (token, 256 columns); kRows tokens per warp, all their loads in
-// flight before the first store.
-constexpr int kFwdRows = 2;
+// One warp per (token rows, 256 columns), all its loads in flight before the
+// first store: as many rows as 16 registers hold, 4 of a bf16 table (65536 x
+// 2048 bf16 70 -> 61 us against 2), 2 of an fp32 one (16384 x 384 9.0 us; 4 rows
+// leave too few warps, 11.2).
+template <typename TW, bool VEC>
+constexpr int fwd_rows() {
+  return 16 / Row8<TW, VEC>::kRegs;
+}
 
-template <typename TW, typename TX, bool VEC>
+template <typename TW, typename TX, bool VEC, bool POS>
 __global__ void __launch_bounds__(256) embed_fwd_kernel(const int* __restrict__ tok, const TW* __restrict__ W, int ldw,
                                                         const float* __restrict__ P, int S, float scale,
                                                         TX* __restrict__ x, int ldx, int n, int d, int V, int slabs) {
+  constexpr int kRows = fwd_rows<TW, VEC>();
   const int lane = threadIdx.x & 31;
-  const long long item = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  const int slab = (int)(item % slabs);
-  const long long i0 = item / slabs * kFwdRows;
-  const int c0 = slab * kSlab, left = d - c0;
-  float v[kFwdRows][8];
+  const unsigned item = blockIdx.x * 8u + (threadIdx.x >> 5);
+  const unsigned group = item / (unsigned)slabs;
+  const int c0 = (int)(item - group * slabs) * kSlab, left = d - c0;
+  const long long i0 = (long long)group * kRows;
+  if (i0 >= n) return;
+  Row8<TW, VEC> w[kRows];
+  Row8<float, VEC> p[POS ? kRows : 1];
 #pragma unroll
-  for (int r = 0; r < kFwdRows; ++r) {
-    const int t = i0 + r < n ? tok[i0 + r] : -1;
-    if (t >= 0 && t < V) {
-      load8<VEC>(W + (size_t)t * ldw + c0, lane, left, v[r]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[r][k] = 0.f;
-    }
+  for (int r = 0; r < kRows; ++r) {
+    const int t = i0 + r < n ? __ldg(tok + i0 + r) : -1;
+    if (POS) p[r].load(P + (size_t)((int)(i0 + r) % S) * d + c0, lane, left);
+    if (t >= 0 && t < V)
+      w[r].load(W + (size_t)t * ldw + c0, lane, left);
+    else
+      w[r].zero();
   }
 #pragma unroll
-  for (int r = 0; r < kFwdRows; ++r) {
+  for (int r = 0; r < kRows; ++r) {
     if (i0 + r >= n) break;
+    float v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[r][k] *= scale;
-    if (P) {
-      float p[8];
-      load8<VEC>(P + (size_t)((int)(i0 + r) % S) * d + c0, lane, left, p);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[r][k] += p[k];
-    }
-    store8<VEC>(x + (size_t)(i0 + r) * ldx + c0, lane, left, v[r]);
+    for (int k = 0; k < 8; ++k) v[k] = POS ? fmaf(scale, w[r].get(k), p[r].get(k)) : scale * w[r].get(k);
+    store8<VEC>(x + (size_t)(i0 + r) * ldx + c0, lane, left, v);
   }
 }
 
 // ---------------------------------------------------------------- token sort
 // Stable LSD radix sort of (token, position) by one cluster: every warp owns a
-// contiguous range of the input. Per pass each warp counts its digits
-// (match-any gives equal digits of 32 keys one representative), the counts are
-// scanned over warps, over the cluster's CTAs (through distributed shared
-// memory) and over digits, and each warp scatters its keys in order. Ids
-// outside [0, V) get the key V and end up last. Afterwards seg[t] is the range
-// of token t in the sorted order (0, 0 where it does not occur).
-constexpr int kSortThreads = 1024, kSortWarps = 32, kMaxDigitBits = 10;
+// contiguous range of the input. Per pass each warp ranks its keys among the
+// equal digits before them (ballots over the digit's bits give the lanes with
+// the same digit), the counts are scanned over warps, over the cluster's CTAs
+// (through distributed shared memory) and over digits, and every key goes to
+// digit base + warp base + rank. Ids outside [0, V) get the key V and end up
+// last. Bound by latency and by the scatter of 8-byte items, about 1.4 cycles
+// per item and SM: 16 CTAs (41 us with 8 at 65536 ids of 18 bits, two passes).
+constexpr int kSortThreads = 1024, kSortWarps = 32, kMaxDigitBits = 9, kMaxCluster = 16;
+constexpr int kBatch = 4;  // keys per lane in registers (65536 keys in 16 CTAs)
 
 struct SortArgs {
   const int* tok;
   int n, V, passes, bits;  // digit bits per pass
   int2* a;                 // [n] (key, position) ping-pong buffers
   int2* b;
-  int2* seg;               // [V]
+  int* rank;               // [n] scratch when a warp's range exceeds one batch
   int* counters;           // [ncounters] cleared for the summing kernel
   int ncounters;
 };
 
-__device__ __forceinline__ int sort_key(const int* tok, int i, int V) {
-  const int t = tok[i];
-  return t >= 0 && t < V ? t : V;
-}
-
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortArgs a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ int hist[];              // [kSortWarps][bins]
   cg::cluster_group cluster = cg::this_cluster();
   const int ncta = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
-  extern __shared__ int hist[];  // [kSortWarps][bins]
   __shared__ int total[1 << kMaxDigitBits];  // this CTA's keys per digit (read by the cluster)
+  __shared__ int base[1 << kMaxDigitBits];   // first place of this CTA's keys per digit
   __shared__ int warp_sums[kSortWarps];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
   const int bins = 1 << a.bits;
   const int gt = cta * kSortThreads + tid, nthreads = ncta * kSortThreads;
-  for (int i = gt; i < a.V; i += nthreads) a.seg[i] = make_int2(0, 0);
-  for (int i = gt; i < a.ncounters; i += nthreads) a.counters[i] = 0;
 
   // this warp's range, a multiple of 32 keys long
   const int warps = ncta * kSortWarps;
   const int per = ((a.n + warps - 1) / warps + 31) & ~31;
-  const int lo = min((long long)a.n, (long long)(cta * kSortWarps + w) * per), hi = min((long long)a.n, (long long)lo + per);
+  const long long lo = min((long long)a.n, (long long)(cta * kSortWarps + w) * per), hi = min((long long)a.n, lo + per);
+  const bool one_batch = per <= 32 * kBatch;
   int* wh = hist + w * bins;
+  const unsigned lt = (1u << lane) - 1;
   const int2* src = nullptr;  // null: the token ids themselves
+  int2 kv[kBatch];
+  int rank[kBatch];
+  auto load = [&](long long i0) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const long long i = i0 + 32 * u + lane;
+      kv[u] = make_int2(0, (int)i);
+      if (i < hi) {
+        if (src) {
+          kv[u] = src[i];
+        } else {
+          const int t = a.tok[i];
+          kv[u].x = t >= 0 && t < a.V ? t : a.V;
+        }
+      }
+    }
+  };
   for (int pass = 0; pass < a.passes; ++pass) {
     const int shift = pass * a.bits;
     int2* dst = pass & 1 ? a.b : a.a;
     for (int i = lane; i < bins; i += 32) wh[i] = 0;
     __syncwarp();
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-      const bool in = i0 + lane < hi;
-      const int key = in ? (src ? src[i0 + lane].x : sort_key(a.tok, i0 + lane, a.V)) : 0;
-      const int digit = in ? (key >> shift) & (bins - 1) : bins;
-      const unsigned same = __match_any_sync(0xffffffffu, digit);
-      if (in && (same & ((1u << lane) - 1)) == 0) wh[digit] += __popc(same);
-      __syncwarp();
+    for (long long i0 = lo; i0 < hi; i0 += 32 * kBatch) {
+      load(i0);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const long long first = i0 + 32 * u;
+        if (first >= hi) break;
+        const bool in = first + lane < hi;
+        const int digit = (kv[u].x >> shift) & (bins - 1);
+        unsigned same = __ballot_sync(0xffffffffu, in);
+        for (int k = 0; k < a.bits; ++k) {
+          const unsigned v = __ballot_sync(0xffffffffu, (digit >> k) & 1);
+          same &= (digit >> k) & 1 ? v : ~v;
+        }
+        if (in) rank[u] = wh[digit] + __popc(same & lt);
+        __syncwarp();
+        if (in && (same & lt) == 0) wh[digit] += __popc(same);
+        __syncwarp();
+        if (!one_batch && in) a.rank[first + lane] = rank[u];
+      }
     }
+    if (pass == 0)  // off the critical path of the loads above
+      for (int i = gt; i < a.ncounters; i += nthreads) a.counters[i] = 0;
     __syncthreads();
     // counts of one digit: exclusive over the warps, total for the CTA
     if (tid < bins) {
       int s = 0;
-#pragma unroll 8
-      for (int i = 0; i < kSortWarps; ++i) {
-        const int c = hist[i * bins + tid];
-        hist[i * bins + tid] = s;
-        s += c;
+#pragma unroll
+      for (int i0 = 0; i0 < kSortWarps; i0 += 8) {
+        int c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = hist[(i0 + i) * bins + tid];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          hist[(i0 + i) * bins + tid] = s;
+          s += c[i];
+        }
       }
       total[tid] = s;
     }
@@ -207,12 +254,15 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortArgs a) {
     // first place of this CTA's keys of digit `tid`: keys of smaller digits
     // in the whole cluster, then of the same digit in earlier CTAs
     int all = 0, before = 0;
-    if (tid < bins)
-      for (int c = 0; c < ncta; ++c) {
-        const int v = cluster.map_shared_rank(total, c)[tid];
-        all += v;
-        before += c < cta ? v : 0;
-      }
+    if (tid < bins) {
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c)
+        if (c < ncta) {
+          const int v = cluster.map_shared_rank(total, c)[tid];
+          all += v;
+          before += c < cta ? v : 0;
+        }
+    }
     int incl = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -221,101 +271,126 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortArgs a) {
     }
     if (lane == 31) warp_sums[w] = incl;
     __syncthreads();
-    if (w == 0) {
-      int v = warp_sums[lane];
+    int earlier = lane < w ? warp_sums[lane] : 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-      }
-      warp_sums[lane] = v;
-    }
+    for (int o = 16; o; o >>= 1) earlier += __shfl_xor_sync(0xffffffffu, earlier, o);
+    if (tid < bins) base[tid] = earlier + incl - all + before;
     __syncthreads();
-    if (tid < bins) {
-      const int base = incl - all + (w ? warp_sums[w - 1] : 0) + before;
-#pragma unroll 8
-      for (int i = 0; i < kSortWarps; ++i) hist[i * bins + tid] += base;
-    }
-    __syncthreads();
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-      const bool in = i0 + lane < hi;
-      int2 kv = make_int2(0, i0 + lane);
-      if (in) {
-        if (src)
-          kv = src[i0 + lane];
-        else
-          kv.x = sort_key(a.tok, i0 + lane, a.V);
+    for (long long i0 = lo; i0 < hi; i0 += 32 * kBatch) {
+      if (!one_batch) {
+        load(i0);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+          if (i0 + 32 * u + lane < hi) rank[u] = a.rank[i0 + 32 * u + lane];
       }
-      const int digit = in ? (kv.x >> shift) & (bins - 1) : bins;
-      const unsigned same = __match_any_sync(0xffffffffu, digit);
-      const unsigned below = same & ((1u << lane) - 1);
-      const int at = in ? wh[digit] + __popc(below) : 0;
-      __syncwarp();
-      if (in) {
-        dst[at] = kv;
-        if (below == 0) wh[digit] += __popc(same);
-      }
-      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (i0 + 32 * u + lane < hi) {
+          const int digit = (kv[u].x >> shift) & (bins - 1);
+          dst[base[digit] + wh[digit] + rank[u]] = kv[u];
+        }
     }
     cluster.sync();  // dst complete; nobody reads `total` any more
     src = dst;
   }
-  for (int i = gt; i < a.n; i += nthreads) {
-    const int key = src[i].x;
-    if (key >= a.V) continue;
-    if (i == 0 || src[i - 1].x != key) a.seg[key].x = i;
-    if (i + 1 == a.n || src[i + 1].x != key) a.seg[key].y = i + 1;
+}
+
+// ---------------------------------------------------------------- rows without a token
+// Zeroes the rows of dW whose token does not occur, on the SMs that the sort's
+// CTAs leave free. The table is cut into groups of 32 rows dealt out in turn to
+// 512 CTAs, all resident (148 took 121 us for 537 MB beside the sort, 512 take
+// 90); a CTA finds the tokens of its groups by reading all ids (4
+// bytes per id and CTA, from L2), so it waits for nothing. The rows go out as
+// bulk copies of a zeroed piece of shared memory, one lane per row. Launched
+// as the sort's dependent; block 0 ends after the sort, so that a kernel that
+// waits for this one waits for both.
+constexpr int kZeroThreads = 512, kZeroCap = 2048;  // groups marked at a time
+constexpr int kZeroBytes = 8192;
+
+struct ZeroArgs {
+  const int* tok;
+  int n, V;
+  char* dW;            // rows of row_bytes, pitch bytes apart
+  size_t pitch;
+  int row_bytes, vec;  // vec: whole 16-byte units
+};
+
+__global__ void __launch_bounds__(kZeroThreads) embed_zero_kernel(ZeroArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ unsigned bits[kZeroCap];
+  __shared__ __align__(128) uint4 zeros[kZeroBytes / 16];
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int G = gridDim.x, lg = 31 - __clz(G);  // a power of two
+  const int groups = (int)(((long long)a.V + 31) / 32);
+  const int mine = (groups - (int)blockIdx.x + G - 1) >> lg;  // groups of this CTA
+  if (a.vec) {
+    for (int i = tid; i < kZeroBytes / 16; i += kZeroThreads) zeros[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
   }
+  for (int g0 = 0; g0 < mine; g0 += kZeroCap) {
+    const int count = min(kZeroCap, mine - g0);
+    __syncthreads();
+    for (int i = tid; i < count; i += kZeroThreads) bits[i] = 0;
+    __syncthreads();
+    auto mark = [&](int t) {
+      const unsigned k = ((unsigned)t >> (5 + lg)) - g0;
+      if ((((unsigned)t >> 5) & (G - 1)) == blockIdx.x && (unsigned)t < (unsigned)a.V && k < (unsigned)count)
+        atomicOr(&bits[k], 1u << (t & 31));
+    };
+    const int n4 = ((uintptr_t)a.tok & 15) ? 0 : a.n >> 2;  // ids four at a time where the array allows
+#pragma unroll 4
+    for (int i = tid; i < n4; i += kZeroThreads) {
+      const int4 t = __ldg(reinterpret_cast<const int4*>(a.tok) + i);
+      mark(t.x);
+      mark(t.y);
+      mark(t.z);
+      mark(t.w);
+    }
+    for (int i = n4 * 4 + tid; i < a.n; i += kZeroThreads) mark(a.tok[i]);
+    __syncthreads();
+    if (a.vec) {
+      for (int k = w; k < count; k += kZeroThreads / 32) {
+        const long long t = ((long long)(g0 + k) * G + blockIdx.x) * 32 + lane;
+        if (t >= a.V || bits[k] >> lane & 1) continue;
+        char* row = a.dW + (size_t)t * a.pitch;
+        for (int j = 0; j < a.row_bytes; j += kZeroBytes)
+          bulk_store(row + j, zeros, (uint32_t)min(kZeroBytes, a.row_bytes - j));
+      }
+    } else {  // elements are 2 or 4 bytes
+      for (int i = w; i < count * 32; i += kZeroThreads / 32) {
+        const long long t = ((long long)(g0 + (i >> 5)) * G + blockIdx.x) * 32 + (i & 31);
+        if (t >= a.V || bits[i >> 5] >> (i & 31) & 1) continue;
+        char* row = a.dW + (size_t)t * a.pitch;
+        for (int j = lane * 2; j < a.row_bytes; j += 64) *reinterpret_cast<uint16_t*>(row + j) = 0;
+      }
+    }
+  }
+  if (a.vec) {
+    bulk_commit();
+    bulk_wait0();
+  }
+  if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- sums
-// A warp owns 256 columns of one table row and adds the token's rows of dx in
-// order. A token that occurs more than 2C times is split at multiples of C in
-// the sorted order: one warp per chunk of C positions sums its part into
-// scratch, and the warp that finishes a token's last outstanding part adds the
-// parts in order. (A chunk touches at most two such tokens: the one its first
-// position belongs to and the one its last position belongs to.)
+// The sorted positions are cut evenly, whatever the tokens: a block owns 128
+// positions and 256 columns, each of its 8 warps 16 positions, so no token's
+// frequency makes a long serial sum. Within its 16 positions a warp adds rows
+// in order and writes the tokens that begin and end there. A token that runs
+// on into the next warp is joined through shared memory, one that runs on into
+// the next block through scratch: the block that finishes the token's last
+// outstanding part adds the parts, all in position order. (A block holds at
+// most two such tokens, one coming in and one going out.)
+constexpr int kWarpPos = 16, kBlockPos = 8 * kWarpPos;
+
 struct SumArgs {
   const int2* sorted;  // (token, position)
-  const int2* seg;
-  int* counters;       // [chunks][slabs] parts finished of the split token that starts in the chunk
-  float* parts;        // [chunks][2][slabs * kSlab]
-  int n, d, V, C, chunks, slabs;
+  int* counters;       // [blocks][slabs] parts finished of the token that runs out of the block it began in
+  float* parts;        // [blocks][2][slabs * kSlab]: of the token coming in, of the one beginning and going out
+  int n, d, V, slabs, blocks;
   int lddx, lddw, accumulate;
   float scale;
 };
-
-// acc += rows of positions [p0, p1), in order; kUnroll rows in flight.
-template <typename TG, bool VEC>
-__device__ __forceinline__ void add_rows(const SumArgs& a, const TG* dx, int c0, int p0, int p1, int lane,
-                                         float (&acc)[8]) {
-  constexpr int kUnroll = 4;
-  const int left = a.d - c0;
-  for (int q0 = p0; q0 < p1; q0 += 32) {
-    const int mine = q0 + lane < p1 ? a.sorted[q0 + lane].y : 0;
-    const int cnt = min(32, p1 - q0);
-    int j = 0;
-    for (; j + kUnroll <= cnt; j += kUnroll) {
-      float v[kUnroll][8];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int i = __shfl_sync(0xffffffffu, mine, j + u);
-        load8<VEC>(dx + (size_t)i * a.lddx + c0, lane, left, v[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] += v[u][k];
-    }
-    for (; j < cnt; ++j) {
-      float v[8];
-      const int i = __shfl_sync(0xffffffffu, mine, j);
-      load8<VEC>(dx + (size_t)i * a.lddx + c0, lane, left, v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) acc[k] += v[k];
-    }
-  }
-}
 
 template <typename TW, bool VEC>
 __device__ __forceinline__ void finish_row(const SumArgs& a, TW* dW, int t, int c0, int lane, float (&acc)[8]) {
@@ -335,56 +410,160 @@ __device__ __forceinline__ void finish_row(const SumArgs& a, TW* dW, int t, int 
   store8<VEC>(o, lane, a.d - c0, acc);
 }
 
-template <typename TG, typename TW, bool VEC>
-__global__ void __launch_bounds__(256) embed_sum_kernel(const TG* __restrict__ dx, TW* __restrict__ dW, SumArgs a) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  long long item = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  const long long nchunk_items = (long long)a.chunks * 2 * a.slabs;
-  float acc[8] = {};
-  if (item < nchunk_items) {  // part of a split token
-    const int slab = (int)(item % a.slabs);
-    item /= a.slabs;
-    const int side = (int)(item & 1), c = (int)(item >> 1);
-    const int first = c * a.C, last = min(a.n, first + a.C) - 1;
-    const int t0 = a.sorted[first].x, t = side ? a.sorted[last].x : t0;
-    if (t >= a.V || (side && t == t0)) return;
-    const int2 sg = a.seg[t];
-    if (sg.y - sg.x <= 2 * a.C) return;
-    const int c0 = slab * kSlab, width = a.slabs * kSlab;
-    add_rows<TG, VEC>(a, dx, c0, max(first, sg.x), min(last + 1, sg.y), lane, acc);
-    float* part = a.parts + ((size_t)c * 2 + side) * width + c0;
+struct SumShared {
+  float head[8][kSlab];  // element k of lane l at [l + 32 k]
+  int through[8];                        // the warp's positions are one token that comes in and goes on
+  int last_token[2], last_block[2], last_parts[2];  // token whose parts are complete (or -1), its blocks
+};
+
+__device__ __forceinline__ void put(float (&row)[kSlab], int lane, const float (&acc)[8]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) part[Lane8<VEC>::col(lane, k)] = acc[k];
+  for (int k = 0; k < 8; ++k) row[lane + 32 * k] = acc[k];
+}
+__device__ __forceinline__ void add(const float (&row)[kSlab], int lane, float (&acc)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) acc[k] += row[lane + 32 * k];
+}
+
+// First block b in [lo, hi) whose position `at` (the last one of the order
+// where the block is short) holds a token >= t, or hi. The warp probes 32
+// blocks at a time: the last of each of 32 equal shares.
+__device__ __forceinline__ int search(const SumArgs& a, int lo, int hi, int at, int t, int lane) {
+  while (lo < hi) {
+    const int step = (hi - lo + 31) / 32, b = lo + (lane + 1) * step - 1;
+    const bool ge = b >= hi || a.sorted[min((long long)a.n - 1, (long long)b * kBlockPos + at)].x >= t;
+    const unsigned m = __ballot_sync(0xffffffffu, ge);
+    if (!m) return hi;
+    lo += (__ffs(m) - 1) * step;
+    hi = min(hi, lo + step - 1);
+  }
+  return lo;
+}
+
+// Writes the block's part of token t and notes the token if that was the last part.
+__device__ __forceinline__ void put_part(const SumArgs& a, SumShared& sh, int blk, int slab, int side, int t, int lane,
+                                         const float (&acc)[8]) {
+  float* p = a.parts + ((size_t)blk * 2 + side) * a.slabs * kSlab + slab * kSlab;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) p[lane + 32 * k] = acc[k];
+  __threadfence();
+  // the token's blocks: from the one it runs out of (its last position's
+  // token) to the last one whose first position has it
+  const int b0 = side ? blk : search(a, 0, blk, kBlockPos - 1, t, lane);
+  const int b1 = search(a, blk + 1, a.blocks, 0, t + 1, lane) - 1;
+  __syncwarp();
+  if (lane == 0 && atomicAdd(&a.counters[(size_t)b0 * a.slabs + slab], 1) == b1 - b0) {
+    sh.last_token[side] = t;
+    sh.last_block[side] = b0;
+    sh.last_parts[side] = b1 - b0 + 1;
+  }
+}
+
+template <typename TG, typename TW, bool VEC>
+__global__ void __launch_bounds__(256, 4) embed_sum_kernel(const TG* __restrict__ dx, TW* __restrict__ dW, SumArgs a) {
+  __shared__ SumShared sh;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int blk = blockIdx.x / a.slabs, slab = blockIdx.x % a.slabs;
+  const int c0 = slab * kSlab, left = a.d - c0;
+  if (threadIdx.x < 2) sh.last_token[threadIdx.x] = -1;
+  // lanes 0..15: this warp's positions, 16: the one after them, 17: the one before
+  const int p0 = blk * kBlockPos + w * kWarpPos;
+  const int pl = lane <= kWarpPos ? p0 + lane : p0 - 1;
+  int2 kv = make_int2(a.V, 0);
+  if (lane <= kWarpPos + 1 && pl >= 0 && pl < a.n) kv = a.sorted[pl];
+  if (lane == kWarpPos + 1 && pl < 0) kv.x = -1;
+  const int cnt = __popc(__ballot_sync(0xffffffffu, lane < kWarpPos && kv.x < a.V));
+  const int before = __shfl_sync(0xffffffffu, kv.x, kWarpPos + 1), after = __shfl_sync(0xffffffffu, kv.x, kWarpPos);
+  int cur = __shfl_sync(0xffffffffu, kv.x, 0);
+  bool coming = before == cur;  // the current token began before this warp's positions
+  bool through = false, tail = false;
+  float acc[8] = {};
+  if (cnt) {
+    // as many rows in flight as 32 registers hold: 8 of bf16, 4 of fp32
+    using Row = Row8<TG, VEC>;
+    constexpr int kUnroll = 32 / Row::kRegs;
+#pragma unroll 1
+    for (int j = 0; j < cnt; j += kUnroll) {
+      Row v[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int i = __shfl_sync(0xffffffffu, kv.y, j + u);
+        if (j + u < cnt) v[u].load(dx + (size_t)i * a.lddx + c0, lane, left);
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int t = __shfl_sync(0xffffffffu, kv.x, j + u);
+        if (j + u >= cnt) break;
+        if (t != cur) {
+          if (coming)
+            put(sh.head[w], lane, acc);
+          else
+            finish_row<TW, VEC>(a, dW, cur, c0, lane, acc);
+          coming = false;
+          cur = t;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += v[u].get(k);
+      }
+    }
+    const bool going = cnt == kWarpPos && after == cur;
+    if (coming) {
+      put(sh.head[w], lane, acc);
+      through = going;
+    } else if (going) {
+      tail = true;  // stays in acc: this warp joins the token
+    } else {
+      finish_row<TW, VEC>(a, dW, cur, c0, lane, acc);
+    }
+  }
+  if (lane == 0) sh.through[w] = through;
+  __syncthreads();
+  if (w == 0 && cnt && before == __shfl_sync(0xffffffffu, kv.x, 0)) {  // the token that comes into the block
+    float in[8] = {};
+    add(sh.head[0], lane, in);
+    for (int i = 0; i < 7 && sh.through[i]; ++i) add(sh.head[i + 1], lane, in);
+    put_part(a, sh, blk, slab, 0, before, lane, in);
+  }
+  if (tail) {  // a token that begins in this warp and goes on
+    int i = w + 1;
+    for (; i < 8; ++i) {
+      add(sh.head[i], lane, acc);
+      if (!sh.through[i]) break;
+    }
+    if (i < 8)
+      finish_row<TW, VEC>(a, dW, cur, c0, lane, acc);
+    else
+      put_part(a, sh, blk, slab, 1, cur, lane, acc);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    const int t = sh.last_token[side];
+    if (t < 0) continue;
+    // every part of the token is written: its blocks, split over the warps
     __threadfence();
-    __syncwarp();
-    const int cs = sg.x / a.C, ce = (sg.y - 1) / a.C;
-    int done = 0;
-    if (lane == 0) done = atomicAdd(&a.counters[(size_t)cs * a.slabs + slab], 1);
-    done = __shfl_sync(0xffffffffu, done, 0);
-    if (done != ce - cs) return;
-    __threadfence();
+    const int b0 = sh.last_block[side], parts = sh.last_parts[side], per = (parts + 7) / 8;
+    const int i1 = min(parts, (w + 1) * per);
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] = 0.f;
 #pragma unroll 4
-    for (int i = cs; i <= ce; ++i) {
-      // side 1 where the token starts inside the chunk
-      const float* p = a.parts + ((size_t)i * 2 + (i == cs && sg.x > cs * a.C ? 1 : 0)) * width + c0;
+    for (int i = w * per; i < i1; ++i) {
+      // where the token began it is that block's outgoing part
+      const float* p = a.parts + ((size_t)(b0 + i) * 2 + (i == 0)) * a.slabs * kSlab + c0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) acc[k] += __ldcg(p + Lane8<VEC>::col(lane, k));
+      for (int k = 0; k < 8; ++k) acc[k] += __ldcg(p + lane + 32 * k);
     }
-    finish_row<TW, VEC>(a, dW, t, c0, lane, acc);
-    return;
+    __syncthreads();
+    put(sh.head[w], lane, acc);
+    __syncthreads();
+    if (w == 0) {
+      for (int i = 1; i < 8; ++i) add(sh.head[i], lane, acc);
+      finish_row<TW, VEC>(a, dW, t, c0, lane, acc);
+    }
   }
-  item -= nchunk_items;
-  const long long t = item / a.slabs;
-  if (t >= a.V) return;
-  const int c0 = (int)(item % a.slabs) * kSlab;
-  const int2 sg = a.seg[t];
-  const int len = sg.y - sg.x;
-  if (len > 2 * a.C || (a.accumulate && len == 0)) return;
-  add_rows<TG, VEC>(a, dx, c0, sg.x, sg.y, lane, acc);
-  finish_row<TW, VEC>(a, dW, (int)t, c0, lane, acc);
 }
 
 bool type_ok(int t) { return t == DGX_F32 || t == DGX_BF16; }
@@ -397,48 +576,67 @@ bool vec_ok(const void* p, int type, int ld, int d) {
 
 size_t align16(size_t b) { return (b + 15) & ~size_t(15); }
 
-// Positions per chunk of a split token: about half of sqrt(n), so that neither
-// one chunk's rows nor one token's parts make a long serial sum.
-int chunk_len(int n) {
-  int c = 32;
-  while (c < 512 && (long long)c * c * 4 < n) c *= 2;
-  return c;
-}
-
 struct Layout {
-  int C, chunks, slabs;
-  size_t a, b, seg, counters, parts, bytes;
+  int blocks, slabs;  // blocks of kBlockPos positions
+  size_t a, b, rank, counters, parts, bytes;
 };
-Layout layout(int n, int d, int V) {
+Layout layout(int n, int d) {
   Layout l;
-  l.C = chunk_len(n);
-  l.chunks = (n + l.C - 1) / l.C;
+  l.blocks = (int)(((long long)n + kBlockPos - 1) / kBlockPos);
   l.slabs = (d + kSlab - 1) / kSlab;
   size_t o = 0;
   l.a = o, o += align16((size_t)n * 8);
   l.b = o, o += align16((size_t)n * 8);
-  l.seg = o, o += align16((size_t)V * 8);
-  l.counters = o, o += align16((size_t)l.chunks * l.slabs * 4);
-  l.parts = o, o += (size_t)l.chunks * 2 * l.slabs * kSlab * 4;
+  l.rank = o, o += align16((size_t)n * 4);
+  l.counters = o, o += align16((size_t)l.blocks * l.slabs * 4);
+  l.parts = o, o += (size_t)l.blocks * 2 * l.slabs * kSlab * 4;
   l.bytes = o;
   return l;
 }
 
-cudaError_t launch_sort(const SortArgs& a, cudaStream_t s) {
-  const int smem = kSortWarps * (1 << a.bits) * 4;
-  cudaError_t e =
-      cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortWarps * 4 << kMaxDigitBits);
-  if (e != cudaSuccess) return e;
+// CTAs of the sorting cluster: 16 where the device can place such a cluster
+// (more than the portable 8), looked up once per device.
+int wide_cluster() {
+  static std::atomic<int> cache[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int c = cache[dev & 63].load(std::memory_order_relaxed);
+  if (c) return c;
+  const int smem = kSortWarps * 4 << kMaxDigitBits;
+  c = 8;
+  int placed = 0;
   cudaLaunchConfig_t cfg{};
-  // up to 4096 tokens one CTA sorts without leaving its SM
-  const int ncta = a.n <= 4096 ? 1 : 8;
-  cfg.gridDim = dim3(ncta);
+  cfg.gridDim = dim3(kMaxCluster);
   cfg.blockDim = dim3(kSortThreads);
   cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kMaxCluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess &&
+      cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+      cudaOccupancyMaxActiveClusters(&placed, embed_sort_kernel, &cfg) == cudaSuccess && placed > 0)
+    c = kMaxCluster;
+  cudaGetLastError();
+  cache[dev & 63].store(c, std::memory_order_relaxed);
+  return c;
+}
+
+cudaError_t launch_sort(const SortArgs& a, cudaStream_t s) {
+  const int wide = wide_cluster();
+  // up to 4096 tokens one CTA sorts without leaving its SM
+  const int cluster = a.n <= 4096 ? 1 : a.n <= 8192 ? 8 : wide;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(cluster);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = kSortWarps * 4 << a.bits;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ncta;
+  attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
@@ -446,19 +644,33 @@ cudaError_t launch_sort(const SortArgs& a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, embed_sort_kernel, a);
 }
 
-template <typename TG, typename TW, bool VEC>
-cudaError_t launch_sum(const void* dx, void* dW, const SumArgs& a, cudaStream_t s) {
-  const long long items = ((long long)a.chunks * 2 + a.V) * a.slabs;
+// A launch that may start while the kernel before it runs (its
+// griddepcontrol.wait orders what has to be).
+template <typename K, typename... A>
+cudaError_t launch_dependent(K kern, int blocks, int threads, cudaStream_t s, A... args) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((items + 7) / 8));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, embed_sum_kernel<TG, TW, VEC>, (const TG*)dx, (TW*)dW, a);
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+cudaError_t launch_zero(const ZeroArgs& a, cudaStream_t s) {
+  // a power of two of CTAs, a group of rows and 64 KB at least for each
+  const long long units = std::min(((long long)a.V * a.row_bytes + 65535) / 65536, ((long long)a.V + 31) / 32);
+  int ctas = 1;
+  while (ctas < 512 && ctas < units) ctas *= 2;
+  return launch_dependent(embed_zero_kernel, ctas, kZeroThreads, s, a);
+}
+
+template <typename TG, typename TW, bool VEC>
+cudaError_t launch_sum(const void* dx, void* dW, const SumArgs& a, int blocks, cudaStream_t s) {
+  return launch_dependent(embed_sum_kernel<TG, TW, VEC>, blocks, 256, s, (const TG*)dx, (TW*)dW, a);
 }
 
 }  // namespace
@@ -478,19 +690,17 @@ dgx_status dgx_embed_fwd(const int* tok, const void* W, dgx_dtype w_type, int ld
   if (n == 0) return DGX_OK;
   if (!tok || !W || !x) return set_error(DGX_EINVAL, "dgx_embed_fwd: null pointer");
   cudaStream_t s = (cudaStream_t)stream;
-  const int slabs = (d + kSlab - 1) / kSlab;
-  const long long blocks = (((long long)n + kFwdRows - 1) / kFwdRows * slabs + 7) / 8;
-  if (blocks > 0x7fffffffll) return set_error(DGX_EINVAL, "dgx_embed_fwd: n=%d d=%d too large", n, d);
   const bool vec = vec_ok(W, w_type, ldw, d) && vec_ok(x, x_type, ldx, d) && (!P || vec_ok(P, DGX_F32, d, d));
+  const int slabs = (d + kSlab - 1) / kSlab;
+  const int rows = vec && w_type == DGX_BF16 ? fwd_rows<__nv_bfloat16, true>() : fwd_rows<float, true>();
+  const long long items = ((long long)n + rows - 1) / rows * slabs;
+  if (items > 0x7fffffffll) return set_error(DGX_EINVAL, "dgx_embed_fwd: n=%d d=%d too large", n, d);
   auto run = [&](auto* w, auto* o) {
     using TW = std::remove_const_t<std::remove_pointer_t<decltype(w)>>;
     using TX = std::remove_pointer_t<decltype(o)>;
-    if (vec)
-      embed_fwd_kernel<TW, TX, true><<<(unsigned)blocks, 256, 0, s>>>(tok, w, ldw, P, P ? S : 1, scale, o, ldx, n, d, V,
-                                                                      slabs);
-    else
-      embed_fwd_kernel<TW, TX, false><<<(unsigned)blocks, 256, 0, s>>>(tok, w, ldw, P, P ? S : 1, scale, o, ldx, n, d,
-                                                                       V, slabs);
+    auto k = vec ? (P ? embed_fwd_kernel<TW, TX, true, true> : embed_fwd_kernel<TW, TX, true, false>)
+                 : (P ? embed_fwd_kernel<TW, TX, false, true> : embed_fwd_kernel<TW, TX, false, false>);
+    k<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(tok, w, ldw, P, P ? S : 1, scale, o, ldx, n, d, V, slabs);
   };
   if (w_type == DGX_F32 && x_type == DGX_F32) run((const float*)W, (float*)x);
   else if (w_type == DGX_F32) run((const float*)W, (__nv_bfloat16*)x);
@@ -501,7 +711,7 @@ dgx_status dgx_embed_fwd(const int* tok, const void* W, dgx_dtype w_type, int ld
 
 size_t dgx_embed_bwd_workspace_size(int n, int d, int V) {
   if (n <= 0 || d <= 0 || V <= 0) return 0;
-  return layout(n, d, V).bytes;
+  return layout(n, d).bytes;
 }
 
 dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int lddx, float scale, void* dW,
@@ -521,9 +731,9 @@ dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int 
     const size_t es = type_size(dw_type);
     return cuda_status(cudaMemset2DAsync(dW, lddw * es, 0, d * es, V, s), "dgx_embed_bwd");
   }
-  const Layout l = layout(n, d, V);
-  if ((((long long)l.chunks * 2 + V) * l.slabs + 7) / 8 > 0x7fffffffll)
-    return set_error(DGX_EINVAL, "dgx_embed_bwd: V=%d d=%d too large", V, d);
+  const Layout l = layout(n, d);
+  if ((long long)l.blocks * l.slabs > 0x7fffffffll)
+    return set_error(DGX_EINVAL, "dgx_embed_bwd: n=%d V=%d d=%d too large", n, V, d);
   char* ws = (char*)workspace;
   if (ws && workspace_bytes < l.bytes)
     return set_error(DGX_ENOMEM, "dgx_embed_bwd: workspace %zu bytes < %zu", workspace_bytes, l.bytes);
@@ -540,22 +750,27 @@ dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int 
   so.bits = (kb + so.passes - 1) / so.passes;
   so.a = (int2*)(ws + l.a);
   so.b = (int2*)(ws + l.b);
-  so.seg = (int2*)(ws + l.seg);
+  so.rank = (int*)(ws + l.rank);
   so.counters = (int*)(ws + l.counters);
-  so.ncounters = l.chunks * l.slabs;
+  so.ncounters = l.blocks * l.slabs;
   cudaError_t e = launch_sort(so, s);
   if (e != cudaSuccess) return cuda_status(e, "dgx_embed_bwd");
+  if (!accumulate) {
+    ZeroArgs z{tok, n, V, (char*)dW, (size_t)lddw * type_size(dw_type), d * type_size(dw_type), 0};
+    z.vec = (((uintptr_t)dW | z.pitch | (size_t)z.row_bytes) & 15) == 0;
+    e = launch_zero(z, s);
+    if (e != cudaSuccess) return cuda_status(e, "dgx_embed_bwd");
+  }
   SumArgs a{};
   a.sorted = so.passes & 1 ? so.a : so.b;
-  a.seg = so.seg;
   a.counters = so.counters;
   a.parts = (float*)(ws + l.parts);
   a.n = n;
   a.d = d;
   a.V = V;
-  a.C = l.C;
-  a.chunks = l.chunks;
   a.slabs = l.slabs;
+  a.blocks = l.blocks;
+  const int blocks = l.blocks * l.slabs;
   a.lddx = lddx;
   a.lddw = lddw;
   a.accumulate = accumulate ? 1 : 0;
@@ -563,14 +778,14 @@ dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int 
   const bool vec = vec_ok(dx, dx_type, lddx, d) && vec_ok(dW, dw_type, lddw, d);
   const bool g32 = dx_type == DGX_F32, w32 = dw_type == DGX_F32;
   if (g32 && w32)
-    e = vec ? launch_sum<float, float, true>(dx, dW, a, s) : launch_sum<float, float, false>(dx, dW, a, s);
+    e = vec ? launch_sum<float, float, true>(dx, dW, a, blocks, s) : launch_sum<float, float, false>(dx, dW, a, blocks, s);
   else if (g32)
-    e = vec ? launch_sum<float, __nv_bfloat16, true>(dx, dW, a, s) : launch_sum<float, __nv_bfloat16, false>(dx, dW, a, s);
+    e = vec ? launch_sum<float, __nv_bfloat16, true>(dx, dW, a, blocks, s) : launch_sum<float, __nv_bfloat16, false>(dx, dW, a, blocks, s);
   else if (w32)
-    e = vec ? launch_sum<__nv_bfloat16, float, true>(dx, dW, a, s) : launch_sum<__nv_bfloat16, float, false>(dx, dW, a, s);
+    e = vec ? launch_sum<__nv_bfloat16, float, true>(dx, dW, a, blocks, s) : launch_sum<__nv_bfloat16, float, false>(dx, dW, a, blocks, s);
   else
-    e = vec ? launch_sum<__nv_bfloat16, __nv_bfloat16, true>(dx, dW, a, s)
-            : launch_sum<__nv_bfloat16, __nv_bfloat16, false>(dx, dW, a, s);
+    e = vec ? launch_sum<__nv_bfloat16, __nv_bfloat16, true>(dx, dW, a, blocks, s)
+            : launch_sum<__nv_bfloat16, __nv_bfloat16, false>(dx, dW, a, blocks, s);
   return cuda_status(e, "dgx_embed_bwd");
 }
 

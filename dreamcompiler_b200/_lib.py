@@ -100,6 +100,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_fns = {}  # name -> bound entry point, filled by load()
 
 
 def load(path: str = LIB_PATH) -> C.CDLL:
@@ -114,6 +115,7 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
+        _fns[name] = fn
     _lib = lib
     return lib
 
@@ -125,4 +127,8 @@ def check(status: int, where: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args), name)
+    if not _fns:
+        load()
+    status = _fns[name](*args)
+    if status:
+        check(status, name)

@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "launch.h"
 #include "sm100.cuh"
 
 namespace dgx {
@@ -644,33 +645,17 @@ cudaError_t launch_sort(const SortArgs& a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, embed_sort_kernel, a);
 }
 
-// A launch that may start while the kernel before it runs (its
-// griddepcontrol.wait orders what has to be).
-template <typename K, typename... A>
-cudaError_t launch_dependent(K kern, int blocks, int threads, cudaStream_t s, A... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(threads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, args...);
-}
-
 cudaError_t launch_zero(const ZeroArgs& a, cudaStream_t s) {
   // a power of two of CTAs, a group of rows and 64 KB at least for each
   const long long units = std::min(((long long)a.V * a.row_bytes + 65535) / 65536, ((long long)a.V + 31) / 32);
   int ctas = 1;
   while (ctas < 512 && ctas < units) ctas *= 2;
-  return launch_dependent(embed_zero_kernel, ctas, kZeroThreads, s, a);
+  return launch_dependent(embed_zero_kernel, ctas, kZeroThreads, 0, 1, s, a);
 }
 
 template <typename TG, typename TW, bool VEC>
 cudaError_t launch_sum(const void* dx, void* dW, const SumArgs& a, int blocks, cudaStream_t s) {
-  return launch_dependent(embed_sum_kernel<TG, TW, VEC>, blocks, 256, s, (const TG*)dx, (TW*)dW, a);
+  return launch_dependent(embed_sum_kernel<TG, TW, VEC>, blocks, 256, 0, 1, s, (const TG*)dx, (TW*)dW, a);
 }
 
 }  // namespace

@@ -17,6 +17,7 @@
 
 #include "gemm.h"
 #include "head.h"
+#include "launch.h"
 #include "sm100.cuh"
 
 namespace dgx {
@@ -35,121 +36,168 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// Every kernel here is launched as its predecessor's programmatic dependent.
+// The ones that another kernel of the same call follows let it start early;
+// the last one of a call does not, so that what the caller issues next starts
+// with the whole call done.
+__device__ __forceinline__ void dependents_may_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- target lists
 // One warp per row: q = softmax(teacher / T) over the entries whose id lies in
 // [0, V), and the entries in ascending order of (id, position), absent ones
 // last (id kNoId, q 0). A teacher logit of -inf has q = 0; a row whose entries
 // are all absent or -inf has live = 0. The rank of an entry is the number of
-// entries before it (K <= 256: at most 8 x 256 comparisons per lane).
-__global__ void head_lists_kernel(const int* __restrict__ idx, const float* __restrict__ teacher, int R, int V, int K,
-                                  float inv_t, int* __restrict__ sid, float* __restrict__ sq,
-                                  float* __restrict__ live, uint16_t* __restrict__ start, int slots) {
-  __shared__ int ids_s[4][kHeadMaxK], sorted_s[4][kHeadMaxK];
+// entries before it, counted four ids per shared-memory load. start[row][s] is
+// the first entry whose id is at least 128 s. KI: entries per lane.
+template <int KI>
+__global__ void __launch_bounds__(128) head_lists_kernel(const int* __restrict__ idx, const float* __restrict__ teacher,
+                                                         int R, int V, int K, float inv_t, int* __restrict__ sid,
+                                                         float* __restrict__ sq, float* __restrict__ live,
+                                                         uint16_t* __restrict__ start, int slots) {
+  __shared__ __align__(16) int ids_s[4][KI * 32], sorted_s[4][KI * 32];
+  dependents_may_start();
+  wait_for_predecessor();
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.x * 4 + w;
   if (row >= R) return;
   int* ids = ids_s[w];
-  const int* ir = idx + (size_t)row * K;
-  const float* tr = teacher + (size_t)row * K;
+  int* sorted = sorted_s[w];
+  int id[KI];
+  float q[KI];
   float mx = -INFINITY;
-  for (int k = lane; k < K; k += 32) {
-    const int id = ir[k];
-    const bool ok = id >= 0 && id < V;
-    ids[k] = ok ? id : kNoId;
-    if (ok) mx = fmaxf(mx, tr[k]);
+#pragma unroll
+  for (int i = 0; i < KI; ++i) {
+    const int k = lane + 32 * i;
+    id[i] = kNoId;
+    q[i] = -INFINITY;
+    if (k < K) {
+      const int v = idx[(size_t)row * K + k];
+      const float l = teacher[(size_t)row * K + k];
+      if (v >= 0 && v < V) {
+        id[i] = v;
+        q[i] = l;
+        mx = fmaxf(mx, l);
+      }
+    }
+    ids[k] = id[i];
   }
   mx = warp_max(mx);
-  float s = 0.f;
-  if (mx != -INFINITY)
-    for (int k = lane; k < K; k += 32)
-      if (ids[k] != kNoId) s += expf((tr[k] - mx) * inv_t);
-  s = warp_sum(s);
-  __syncwarp();
   const bool any = mx != -INFINITY;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < KI; ++i) {
+    q[i] = any && id[i] != kNoId ? expf((q[i] - mx) * inv_t) : 0.f;
+    s += q[i];
+  }
+  s = warp_sum(s);
   const float inv_s = any ? 1.f / s : 0.f;
-  for (int k = lane; k < K; k += 32) {
-    const int id = ids[k];
-    int rank = 0;
-    for (int j = 0; j < K; ++j) rank += (ids[j] < id || (ids[j] == id && j < k)) ? 1 : 0;
-    const float q = (any && id != kNoId) ? expf((tr[k] - mx) * inv_t) * inv_s : 0.f;
-    sid[(size_t)row * K + rank] = id;
-    sq[(size_t)row * K + rank] = q;
-    sorted_s[w][rank] = id;
+  __syncwarp();
+  int rank[KI] = {};
+#pragma unroll 4
+  for (int j = 0; j < KI * 32; j += 4) {
+    const int4 o = *reinterpret_cast<const int4*>(ids + j);
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int k = lane + 32 * i;
+      rank[i] += (o.x < id[i] || (o.x == id[i] && j < k)) + (o.y < id[i] || (o.y == id[i] && j + 1 < k)) +
+                 (o.z < id[i] || (o.z == id[i] && j + 2 < k)) + (o.w < id[i] || (o.w == id[i] && j + 3 < k));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < KI; ++i) {
+    sorted[rank[i]] = id[i];
+    if (rank[i] < K) {
+      sid[(size_t)row * K + rank[i]] = id[i];
+      sq[(size_t)row * K + rank[i]] = q[i] * inv_s;
+    }
   }
   if (lane == 0) live[row] = any ? 1.f : 0.f;
   __syncwarp();
   for (int t = lane; t < slots; t += 32) {
-    int lo = 0, hi = K;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (sorted_s[w][mid] < t * 128)
-        lo = mid + 1;
-      else
-        hi = mid;
-    }
-    start[(size_t)row * slots + t] = (uint16_t)lo;
+    int lo = 0;  // entries below 128 t: a binary descent over KI * 32 entries
+#pragma unroll
+    for (int step = KI * 32; step; step >>= 1)
+      if (lo + step <= KI * 32 && sorted[lo + step - 1] < t * 128) lo += step;
+    start[(size_t)row * slots + t] = (uint16_t)min(lo, K);
   }
 }
 
 // ---------------------------------------------------------------- forward
 // lse and loss from the statistics part[slot][R] (max of the raw logits and
-// sum of exp((z - max) / T) over 128 columns each). A block owns 32 rows, one
-// per lane; its 32 warps walk the slots and their results are joined through
-// shared memory in a fixed order. Hard target: sq == null.
-__global__ void __launch_bounds__(1024) head_finish_kernel(
+// sum of exp((z - max) / T) over the slot's columns). A block owns 32 rows, one
+// per lane; its NW warps walk the slots, eight loads in flight, and their
+// results are joined in warp order. Hard target: sq == null.
+template <int NW>
+__global__ void __launch_bounds__(NW * 32) head_finish_kernel(
     const float2* __restrict__ part, int slots, int R, int V, float t, float inv_t, const int* __restrict__ sid,
     const float* __restrict__ sq, int K, const float* __restrict__ zs, float* __restrict__ loss,
     float* __restrict__ lse) {
-  __shared__ float2 ms[32][33];
+  __shared__ float2 ms[NW][32];
+  __shared__ float base_s[32], logs_s[32];
+  wait_for_predecessor();
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row0 = blockIdx.x * 32;
-  auto join = [inv_t](float& m, float& s, float m2, float s2) {
-    const float mn = fmaxf(m, m2), base = mn == -INFINITY ? 0.f : mn;
-    s = s * expf((m - base) * inv_t) + s2 * expf((m2 - base) * inv_t);
-    m = mn;
-  };
+  const int row0 = blockIdx.x * 32, row = row0 + lane;
   float m = -INFINITY, s = 0.f;
-  if (row0 + lane < R)
-    for (int i = w; i < slots; i += 32) {
-      const float2 p = part[(size_t)i * R + row0 + lane];
-      join(m, s, p.x, p.y);
+  if (row < R)
+    for (int i = w; i < slots; i += 8 * NW) {
+      float2 p[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        p[u] = i + u * NW < slots ? part[(size_t)(i + u * NW) * R + row] : make_float2(-INFINITY, 0.f);
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) mn = fmaxf(mn, p[u].x);
+      const float base = mn == -INFINITY ? 0.f : mn;
+      s *= expf((m - base) * inv_t);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += p[u].y * expf((p[u].x - base) * inv_t);
+      m = mn;
     }
   ms[w][lane] = make_float2(m, s);
   __syncthreads();
-  // warp w finishes row row0 + w: lane i holds warp i's part
-  const int row = row0 + w;
-  if (row >= R) return;
-  m = ms[lane][w].x;
-  s = ms[lane][w].y;
+  if (w == 0) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    join(m, s, m2, s2);
+    for (int i = 1; i < NW; ++i) m = fmaxf(m, ms[i][lane].x);
+    const float base = m == -INFINITY ? 0.f : m;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) s += ms[i][lane].y * expf((ms[i][lane].x - base) * inv_t);
+    const float log_s = logf(s);
+    if (row < R) lse[row] = base * inv_t + log_s;
+    if (!sq) {
+      // z - lse = (raw - max)/T - log s: subtracting the maximum first keeps
+      // the loss accurate when the logits are large
+      if (row < R) {
+        const int id = sid[row];
+        loss[row] = id >= 0 && id < V ? log_s - (zs[row] - base) * inv_t : 0.f;
+      }
+    } else {
+      base_s[lane] = base;
+      logs_s[lane] = log_s;
+    }
   }
-  // lanes may differ in the last bit of s (the two sides add in either order)
-  s = __shfl_sync(0xffffffffu, s, 0);
-  const float base = m == -INFINITY ? 0.f : m, log_s = logf(s);
-  // z - lse = (raw - max)/T - log s: subtracting the maximum first keeps the
-  // loss accurate when the logits are large
-  float l = 0.f;
-  for (int k = lane; k < K; k += 32) {
-    const int id = sid[(size_t)row * K + k];
-    if (id < 0 || id >= V) continue;
-    const float q = sq ? sq[(size_t)row * K + k] : 1.f;
-    if (q == 0.f) continue;
-    const float lp = (zs[(size_t)row * K + k] - base) * inv_t - log_s;
-    l += sq ? q * (logf(q) - lp) : -lp;
-  }
-  l = warp_sum(l);
-  if (lane == 0) {
-    lse[row] = base * inv_t + log_s;
-    loss[row] = t * t * l;
+  if (!sq) return;
+  __syncthreads();
+  for (int r = w; r < 32 && row0 + r < R; r += NW) {
+    const size_t at = (size_t)(row0 + r) * K;
+    float l = 0.f;
+    for (int k = lane; k < K; k += 32) {
+      const float q = sq[at + k];
+      if (sid[at + k] == kNoId || q == 0.f) continue;
+      l += q * (logf(q) - ((zs[at + k] - base_s[r]) * inv_t - logs_s[r]));
+    }
+    l = warp_sum(l);
+    if (lane == 0) loss[row0 + r] = t * t * l;
   }
 }
 
 // *mean = sum(loss) / R in a fixed order (one block).
 __global__ void head_mean_kernel(const float* __restrict__ loss, int R, float* __restrict__ mean) {
   __shared__ float red[32];
+  wait_for_predecessor();
   float s = 0.f;
   for (int i = threadIdx.x; i < R; i += blockDim.x) s += loss[i];
   s = warp_sum(s);
@@ -164,14 +212,27 @@ __global__ void head_mean_kernel(const float* __restrict__ loss, int R, float* _
 // ---------------------------------------------------------------- backward
 constexpr int kSlabRows = 32;  // rows per partial column sum
 
-// db[j] (+)= scale * sum over slabs of dbp[slab][j], in order.
-__global__ void head_db_kernel(const float* __restrict__ dbp, int slabs, int n, float scale, int accumulate,
-                               float* __restrict__ db) {
-  const int j = blockIdx.x * blockDim.x + threadIdx.x;
-  if (j >= n) return;
+// db[j] (+)= scale * sum over slabs of dbp[slab][j]: a block owns 32 columns, its
+// 8 warps take the slabs in turn and are joined in warp order.
+__global__ void __launch_bounds__(256) head_db_kernel(const float* __restrict__ dbp, int slabs, int n, float scale,
+                                                      int accumulate, float* __restrict__ db) {
+  __shared__ float red[8][32];
+  dependents_may_start();
+  wait_for_predecessor();
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int j = blockIdx.x * 32 + lane;
   float s = 0.f;
-  for (int i = 0; i < slabs; ++i) s += dbp[(size_t)i * n + j];
-  db[j] = (accumulate ? db[j] : 0.f) + scale * s;
+  if (j < n) {
+#pragma unroll 8
+    for (int i = w; i < slabs; i += 8) s += dbp[(size_t)i * n + j];
+  }
+  red[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && j < n) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += red[i][lane];
+    db[j] = (accumulate ? db[j] : 0.f) + scale * s;
+  }
 }
 
 // out[r][j] (+)= scale * sum over slices of acc[slice][r][j], in order, rounded
@@ -179,6 +240,7 @@ __global__ void head_db_kernel(const float* __restrict__ dbp, int slabs, int n, 
 // four elements).
 __global__ void head_out_kernel(const float* __restrict__ acc, int slices, int rows, int d, int lda, float scale,
                                 int bf16_out, int accumulate, void* __restrict__ out, int ldo) {
+  wait_for_predecessor();
   const int dq = (d + 3) >> 2;
   const long long total = (long long)rows * dq;
   const size_t slice = (size_t)rows * lda;
@@ -238,21 +300,25 @@ size_t list_bytes(int R, int V, int K) {
 }
 
 // Sorted target lists of the soft target (the hard one is its own list).
-void target_lists(const HeadArgs& a, Carve& c, HeadTcArgs& t, cudaStream_t s) {
+cudaError_t target_lists(const HeadArgs& a, Carve& c, HeadTcArgs& t, cudaStream_t s) {
   t.sid = a.idx;
   t.K = a.K;
-  if (!a.teacher) return;
+  if (!a.teacher) return cudaSuccess;
   int* si = c.take<int>((size_t)a.R * a.K);
   float* q = c.take<float>((size_t)a.R * a.K);
   float* live = c.take<float>(a.R);
   t.slots = num_slots(a.V);
   uint16_t* start = c.take<uint16_t>((size_t)a.R * t.slots);
-  head_lists_kernel<<<(a.R + 3) / 4, 128, 0, s>>>(a.idx, a.teacher, a.R, a.V, a.K, a.inv_t, si, q, live, start,
-                                                  t.slots);
   t.sid = si;
   t.sq = q;
   t.live = live;
   t.start = start;
+  auto kern = a.K <= 32    ? head_lists_kernel<1>
+              : a.K <= 64  ? head_lists_kernel<2>
+              : a.K <= 128 ? head_lists_kernel<4>
+                           : head_lists_kernel<8>;
+  return launch_dependent(kern, (a.R + 3) / 4, 128, 0, 1, s, a.idx, a.teacher, a.R, a.V, a.K, a.inv_t, si, q, live, start,
+                          t.slots);
 }
 
 HeadTcArgs tc_args(const HeadArgs& a) {
@@ -270,8 +336,7 @@ HeadTcArgs tc_args(const HeadArgs& a) {
 }  // namespace
 
 size_t head_fwd_scratch_bytes(int R, int V, int d, int K, bool lists) {
-  (void)d;
-  const int slots = (V + 127) / 128;
+  const int slots = std::max((V + 127) / 128, lists ? 0 : head_small_slots(R, V, d));
   return align128((size_t)slots * R * 8) + align128((size_t)R * K * 4) + (lists ? list_bytes(R, V, K) : 0);
 }
 
@@ -301,19 +366,33 @@ size_t head_bwd_scratch_bytes(int R, int V, int d, int K, bool lists) {
 }
 
 dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s) {
-  const int slots = (a.V + 127) / 128;
   Carve c{(char*)ws};
   HeadTcArgs t = tc_args(a);
+  const int small = a.teacher ? 0 : head_small_slots(a.R, a.V, a.d);
+  const int slots = small ? small : (a.V + 127) / 128;
   t.part = c.take<float2>((size_t)slots * a.R);
   t.zs = c.take<float>((size_t)a.R * a.K);
   t.n = a.V;
-  target_lists(a, c, t, s);
-  const cudaError_t e = head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, false, nullptr, 0, s);
-  if (e != cudaSuccess) return cuda_status(e, "head forward");
-  head_finish_kernel<<<(a.R + 31) / 32, 1024, 0, s>>>(t.part, slots, a.R, a.V, a.t, a.inv_t, t.sid, t.sq, a.K, t.zs,
-                                                      a.loss, a.lse);
-  if (a.mean) head_mean_kernel<<<1, 1024, 0, s>>>(a.loss, a.R, a.mean);
-  return cuda_status(cudaGetLastError(), "head forward");
+  cudaError_t e = target_lists(a, c, t, s);
+  if (e == cudaSuccess)
+    e = small ? head_small(t, a.H, a.ldh, a.W, a.ldw, small, s)
+              : head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, false, nullptr, 0, s);
+  if (e == cudaSuccess) {
+    // few slots: few warps, so that many rows do not pay for idle ones
+    const bool wide = slots > 32;
+    e = launch_dependent(wide ? head_finish_kernel<32> : head_finish_kernel<4>, (a.R + 31) / 32, wide ? 1024 : 128, 0, 1,
+                         s, t.part, slots, a.R, a.V, a.t, a.inv_t, t.sid, t.sq, a.K, t.zs, a.loss, a.lse);
+  }
+  if (e == cudaSuccess && a.mean) e = launch_dependent(head_mean_kernel, 1, 1024, 0, 1, s, a.loss, a.R, a.mean);
+  return cuda_status(e, "head forward");
+}
+
+static cudaError_t launch_out(const float* acc, int slices, int rows, const HeadArgs& a, int lda, int bf16_out,
+                              int accumulate, void* out, int ldo, cudaStream_t s) {
+  const long long quads = (long long)rows * ((a.d + 3) / 4);
+  const unsigned blocks = (unsigned)std::min<long long>((quads + 255) / 256, num_sms() * 8ll);
+  return launch_dependent(head_out_kernel, blocks, 256, 0, 1, s, acc, slices, rows, a.d, lda, a.scale, bf16_out,
+                          accumulate, out, ldo);
 }
 
 dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
@@ -324,18 +403,22 @@ dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
   float* dbp = c.take<float>((size_t)p.slabs * p.pc);
   float* dh = p.dh_scratch ? c.take<float>((size_t)p.sp.dh * a.R * p.dp) : nullptr;
   float* dw = p.sp.dw > 1 ? c.take<float>((size_t)p.sp.dw * std::min(p.pc, a.V) * p.dp) : nullptr;
-  target_lists(a, c, t, s);
+  cudaError_t e = target_lists(a, c, t, s);
+  if (e != cudaSuccess) return cuda_status(e, "head backward");
   t.dbp = a.db ? dbp : nullptr;
   t.dloss = a.dloss;
   t.lse = a.lse;
-  const int grid_out = num_sms() * 8;
   for (int c0 = 0; c0 < a.V; c0 += p.pc) {
     const int n = std::min(p.pc, a.V - c0);
     t.c0 = c0;
     t.n = n;
-    cudaError_t e = head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, true, g, p.pc, s);
+    e = head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, true, g, p.pc, s);
     if (e != cudaSuccess) return cuda_status(e, "head backward");
-    if (a.db) head_db_kernel<<<(n + 255) / 256, 256, 0, s>>>(dbp, p.slabs, n, a.scale, a.accumulate, a.db + c0);
+    if (a.db) {
+      e = launch_dependent(head_db_kernel, (n + 31) / 32, 256, 0, 1, s, dbp, p.slabs, n, a.scale, a.accumulate,
+                           a.db + c0);
+      if (e != cudaSuccess) return cuda_status(e, "head backward");
+    }
     HeadGradTc m{};
     m.G = g;
     m.ldg = p.pc;
@@ -351,11 +434,11 @@ dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
     if (a.dH) m.out[0] = dh ? GradOut{dh, 0, c0 > 0, p.dp, p.sp.dh, 1.f} : GradOut{a.dH, a.dh_bf16, 0, a.lddh, 1, a.scale};
     if (a.dW) m.out[1] = dw ? GradOut{dw, 0, 0, p.dp, p.sp.dw, 1.f} : GradOut{dw_out, a.dw_bf16, a.accumulate, a.lddw, 1, a.scale};
     e = head_grads_tc(m, s);
+    if (e == cudaSuccess && a.dW && dw) e = launch_out(dw, p.sp.dw, n, a, p.dp, a.dw_bf16, a.accumulate, dw_out, a.lddw, s);
     if (e != cudaSuccess) return cuda_status(e, "head backward");
-    if (a.dW && dw) head_out_kernel<<<grid_out, 256, 0, s>>>(dw, p.sp.dw, n, a.d, p.dp, a.scale, a.dw_bf16, a.accumulate, dw_out, a.lddw);
   }
-  if (a.dH && dh) head_out_kernel<<<grid_out, 256, 0, s>>>(dh, p.sp.dh, a.R, a.d, p.dp, a.scale, a.dh_bf16, 0, a.dH, a.lddh);
-  return cuda_status(cudaGetLastError(), "head backward");
+  if (a.dH && dh) e = launch_out(dh, p.sp.dh, a.R, a, p.dp, a.dh_bf16, 0, a.dH, a.lddh, s);
+  return cuda_status(e, "head backward");
 }
 
 }  // namespace dgx

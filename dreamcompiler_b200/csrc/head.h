@@ -60,6 +60,12 @@ struct HeadTcArgs {
 cudaError_t head_logits_tc(HeadTcArgs a, const void* H, int ldh, const void* W, int ldw, bool grad, void* g, int ldg,
                            cudaStream_t s);
 
+// The forward's statistics for up to 32 rows and a hard target (head_small.cu):
+// part [slots][R] and zs [R], with slots = head_small_slots() (0: not for these
+// sizes).
+int head_small_slots(int R, int V, int d);
+cudaError_t head_small(const HeadTcArgs& a, const void* H, int ldh, const void* W, int ldw, int slots, cudaStream_t s);
+
 // Both gradient products of one piece (head_grads.cu). out[0] is dH [R][ld],
 // out[1] dW [n][ld]; with splits > 1 the output is fp32 partial sums
 // [splits][rows][ld]. ptr null: the product is skipped.

@@ -17,6 +17,7 @@
 
 #include "gemm.h"
 #include "head.h"
+#include "launch.h"
 #include "pair.cuh"
 #include "sm100.cuh"
 
@@ -131,6 +132,7 @@ __global__ void __launch_bounds__(HG_THREADS, 1)
   cluster_sync_all2();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
   if (warp == 0) {
@@ -288,22 +290,11 @@ bool encode_out(CUtensorMap* map, void* base, bool bf16, uint64_t d, uint64_t ro
 
 template <int BN>
 cudaError_t launch(const CUtensorMap (&m)[6], const GradArgs& a, int pairs, cudaStream_t s) {
-  cudaError_t e =
-      cudaFuncSetAttribute(head_grads_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, HgCfg<BN>::SMEM);
+  static std::atomic<unsigned long long> done;
+  const cudaError_t e = allow_smem(head_grads_kernel<BN>, HgCfg<BN>::SMEM, done);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(2 * pairs);
-  cfg.blockDim = dim3(HG_THREADS);
-  cfg.dynamicSmemBytes = HgCfg<BN>::SMEM;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, head_grads_kernel<BN>, m[0], m[1], m[2], m[3], m[4], m[5], a);
+  return launch_dependent(head_grads_kernel<BN>, 2 * pairs, HG_THREADS, HgCfg<BN>::SMEM, 2, s, m[0], m[1], m[2], m[3],
+                          m[4], m[5], a);
 }
 
 }  // namespace

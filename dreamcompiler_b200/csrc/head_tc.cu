@@ -15,6 +15,7 @@
 
 #include "gemm.h"
 #include "head.h"
+#include "launch.h"
 #include "pair.cuh"
 #include "sm100.cuh"
 
@@ -97,6 +98,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
   cluster_sync_all2();  // both CTAs' barriers are initialised before any cross-CTA traffic
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const int num_tiles = a.tiles_m * a.tiles_n;
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
@@ -340,26 +343,6 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
   }
 }
 
-template <typename K>
-cudaError_t launch_pairs(K kern, int pairs, cudaStream_t s, const CUtensorMap& h, const CUtensorMap& w,
-                         const CUtensorMap& g, const HeadTcArgs& a) {
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, HD_SMEM);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(2 * pairs);
-  cfg.blockDim = dim3(HD_THREADS);
-  cfg.dynamicSmemBytes = HD_SMEM;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, h, w, g, a);
-}
-
 }  // namespace
 
 // Logits of the piece [c0, c0 + n) of the vocabulary: row statistics
@@ -375,8 +358,11 @@ cudaError_t head_logits_tc(HeadTcArgs a, const void* H, int ldh, const void* W, 
   a.tiles_m = (a.R + 2 * HD_BM - 1) / (2 * HD_BM);
   a.tiles_n = (a.n + HD_BN - 1) / HD_BN;
   const int pairs = (int)std::min<long long>((long long)a.tiles_m * a.tiles_n, num_sms() / 2);
-  return grad ? launch_pairs(head_logits_kernel<kGrad>, pairs, s, mh, mw, mg, a)
-              : launch_pairs(head_logits_kernel<kStats>, pairs, s, mh, mw, mg, a);
+  auto kern = grad ? head_logits_kernel<kGrad> : head_logits_kernel<kStats>;
+  static std::atomic<unsigned long long> done[2];
+  const cudaError_t e = allow_smem(kern, HD_SMEM, done[grad]);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(kern, 2 * pairs, HD_THREADS, HD_SMEM, 2, s, mh, mw, mg, a);
 }
 
 }  // namespace dgx

@@ -150,14 +150,14 @@ __global__ void __launch_bounds__(kWarps * 32) head_small_kernel(const __nv_bflo
   }
 }
 
-int small_smem(int R, int d) { return (d + 31) / 32 * ((R + 7) / 8 > 2 ? 4 : (R + 7) / 8) * 512; }
+int small_smem(int R, int d) { return (d + 31) / 32 * ((R + 7) / 8) * 512; }
 
 }  // namespace
 
 // Statistics slots (blocks) of the small kernel, 0 where it does not apply: up
 // to 32 rows whose fragments fit 96 KB of shared memory (two blocks per SM).
 int head_small_slots(int R, int V, int d) {
-  if (R > 32 || small_smem(R, d) > 96 * 1024) return 0;
+  if (R > 16 || small_smem(R, d) > 96 * 1024) return 0;
   const int tiles = (V + kTileRows - 1) / kTileRows;
   return std::min((tiles + kWarps - 1) / kWarps, 2 * num_sms());
 }
@@ -170,10 +170,8 @@ cudaError_t head_small(const HeadTcArgs& a, const void* H, int ldh, const void* 
     return launch_dependent(kern, slots, kWarps * 32, smem, 1, s, (const __nv_bfloat16*)H, ldh, (const __nv_bfloat16*)W,
                             ldw, a.bias, a.sid, a.R, a.V, a.d, a.zs, a.part);
   };
-  static std::atomic<unsigned long long> done[3];
-  if (a.R <= 8) return run(head_small_kernel<1>, done[0]);
-  if (a.R <= 16) return run(head_small_kernel<2>, done[1]);
-  return run(head_small_kernel<4>, done[2]);
+  static std::atomic<unsigned long long> done[2];
+  return a.R <= 8 ? run(head_small_kernel<1>, done[0]) : run(head_small_kernel<2>, done[1]);
 }
 
 }  // namespace dgx

@@ -26,13 +26,20 @@ constexpr int HD_BM = 128;  // rows per CTA (256 per pair)
 constexpr int HD_BN = 256;  // vocabulary columns per tile (128 W rows loaded per CTA)
 constexpr int HD_BK = 64;   // one 128-byte swizzled row of bf16
 constexpr int HD_STAGE = 2 * HD_BM * HD_BK * 2;  // 16 KB of H and 16 KB of W
-constexpr int HD_STAGES = 6;
 constexpr int HD_EPI_WARPS = 8;
 constexpr int HD_THREADS = 64 + 32 * HD_EPI_WARPS;
-constexpr int HD_SMEM = HD_STAGES * HD_STAGE + HD_EPI_WARPS * 4096 + 1024 + 256;
 constexpr uint32_t HD_TMEM_COLS = 512;
 
 constexpr int kStats = 0, kGrad = 1;
+// Per epilogue warp, after the operand stages: a 4 KB staging box for G (the
+// gradient), and the bias of its 128 columns. Both and six stages do not fit.
+template <int MODE, bool BIAS>
+struct HdCfg {
+  static constexpr int STAGES = MODE == kGrad && BIAS ? 5 : 6;
+  static constexpr int OUT = MODE == kGrad ? HD_EPI_WARPS * 4096 : 0;
+  static constexpr int BIAS_BYTES = BIAS ? HD_EPI_WARPS * 512 : 0;
+  static constexpr int SMEM = STAGES * HD_STAGE + OUT + BIAS_BYTES + 1024 + 256;
+};
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -41,26 +48,119 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// One row's sparse target inside one tile: the entries of its sorted list from
-// the first id of this warp's columns on.
+// One row's sparse target: the entries of its sorted list from a tile's first
+// column on. The entry after the current one is already loaded when the current
+// one is used, so a hit does not wait for memory.
 struct Target {
   const int* ids;   // [K] ascending
   const float* qs;  // [K], or null: every q is 1
-  int k, K, nid;    // next entry and its id (INT_MAX: none)
+  int k, K;         // current entry
+  int nid, pid;     // its id and the following one's (kNone: none)
+  float nq, pq;     // their probabilities
+  static constexpr int kNone = 0x7fffffff;
+  __device__ __forceinline__ void fetch(int i, int& id, float& q) const {
+    id = i < K ? __ldg(ids + i) : kNone;
+    q = i < K && qs ? __ldg(qs + i) : 1.f;
+  }
+  __device__ __forceinline__ void start(int first) {
+    k = first;
+    fetch(k, nid, nq);
+    fetch(k + 1, pid, pq);
+  }
   __device__ __forceinline__ void next() {
     ++k;
-    nid = k < K ? ids[k] : 0x7fffffff;
+    nid = pid;
+    nq = pq;
+    fetch(k + 1, pid, pq);
   }
 };
 
-template <int MODE>
+// Row statistics of 32 logits of one row: the target's logits to zs, the
+// running maximum and sum. n0: column within the piece, j0: its vocabulary id.
+__device__ __forceinline__ void stats32(float (&z)[32], int n0, int j0, int row, const HeadTcArgs& a, Target& tg,
+                                        float& m, float& s) {
+  if (n0 + 32 > a.n) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (n0 + j >= a.n) z[j] = -INFINITY;
+  }
+  while (__any_sync(0xffffffffu, (unsigned)tg.nid - (unsigned)j0 < 32u)) {
+    const int at = (int)((unsigned)tg.nid - (unsigned)j0);
+    float v = 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v = at == j ? z[j] : v;
+    if ((unsigned)at < 32u) {
+      a.zs[(size_t)row * a.K + tg.k] = v;
+      tg.next();
+    }
+  }
+  float cm = max3f(z[0], z[1], z[2]);
+#pragma unroll
+  for (int j = 3; j < 31; j += 2) cm = max3f(cm, z[j], z[j + 1]);
+  cm = fmaxf(cm, z[31]);
+  const float mn = fmaxf(m, cm);
+  const float base = mn == -INFINITY ? 0.f : mn;
+  float2 s0 = make_float2(s * ex2((m - base) * a.k), 0.f), s1 = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    // subtract before scaling: exact for equal logits of any size
+    const float2 x = fsubmul2(z[j], z[j + 1], base, base, a.k, a.k);
+    const float2 y = fsubmul2(z[j + 2], z[j + 3], base, base, a.k, a.k);
+    s0 = fadd2(s0, ex2(x.x), ex2(x.y));
+    s1 = fadd2(s1, ex2(y.x), ex2(y.y));
+  }
+  s = (s0.x + s0.y) + (s1.x + s1.y);
+  m = mn;
+}
+
+// 32 logits of one row to w (exp(z / T - lse) - q). A row without a target
+// (w = 0) is exactly zero, whatever its logits hold.
+__device__ __forceinline__ void grad32(float (&z)[32], int j0, const HeadTcArgs& a, Target& tg, float w, float lse) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    const float2 x = ffma2(z[j], z[j + 1], a.inv_t, -lse);
+    z[j] = ex2(x.x * kLog2e) * w;
+    z[j + 1] = ex2(x.y * kLog2e) * w;
+  }
+  if (w == 0.f) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) z[j] = 0.f;
+  }
+  while (__any_sync(0xffffffffu, (unsigned)tg.nid - (unsigned)j0 < 32u)) {
+    const int at = (int)((unsigned)tg.nid - (unsigned)j0);
+    const bool hit = (unsigned)at < 32u;
+    const float qw = hit ? tg.nq * w : 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) z[j] -= at == j ? qw : 0.f;
+    if (hit) tg.next();
+  }
+}
+
+// Column sums over the warp's 32 rows: 32 x 32 values, each step exchanging
+// half of what is left with the lane 16, 8, ... away; lane j ends with column j
+// in z[0] (31 shuffles instead of 160).
+__device__ __forceinline__ void column_sums(float (&z)[32], int lane) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int j = 0; j < o; ++j) {
+      const float mine = up ? z[j + o] : z[j], give = up ? z[j] : z[j + o];
+      z[j] = mine + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+}
+
+template <int MODE, bool BIAS>
 __global__ void __launch_bounds__(HD_THREADS, 1)
     head_logits_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW,
                        const __grid_constant__ CUtensorMap tmG, HeadTcArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  using Cfg = HdCfg<MODE, BIAS>;
+  constexpr int HD_STAGES = Cfg::STAGES;
   uint8_t* out_stage = smem + HD_STAGES * HD_STAGE;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_stage + HD_EPI_WARPS * 4096);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_stage + Cfg::OUT + Cfg::BIAS_BYTES);
   uint64_t* empty_bar = full_bar + HD_STAGES;
   uint64_t* accf_bar = empty_bar + HD_STAGES;  // [2]
   uint64_t* acce_bar = accf_bar + 2;           // [2]
@@ -174,6 +274,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
     const int q = warp & 3;              // TMEM lane quarter this warp may access
     const int half = (warp - 2) >> 2;    // its 128 columns of the tile
     uint8_t* st = out_stage + (warp - 2) * 4096;
+    float* bias_s = reinterpret_cast<float*>(out_stage + Cfg::OUT) + (warp - 2) * 128;
     uint32_t issued = 0, use = 0;
     for (int t = pair; t < num_tiles; t += npairs, ++use) {
       const int buf = use & 1;
@@ -183,14 +284,13 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
       const int nbase = tn * HD_BN + half * 128;  // first column of this warp, within the piece
       const bool row_ok = row < a.R;
       // the row's target entries from this warp's columns on
-      Target tg{nullptr, nullptr, 0, 0, 0x7fffffff};
+      Target tg{nullptr, nullptr, 0, 0, Target::kNone, Target::kNone, 0.f, 0.f};
       float w = 1.f, lse = 0.f;
       if (row_ok) {
         tg.ids = a.sid + (size_t)row * a.K;
         tg.qs = a.sq ? a.sq + (size_t)row * a.K : nullptr;
         tg.K = a.K;
-        tg.k = (a.start ? a.start[(size_t)row * a.slots + (a.c0 + nbase) / 128] : 0) - 1;
-        tg.next();
+        tg.start(a.start ? a.start[(size_t)row * a.slots + (a.c0 + nbase) / 128] : 0);
         if (MODE == kGrad) {
           const bool live = a.live ? a.live[row] != 0.f : (tg.nid >= 0 && tg.nid < a.V);
           w = live ? (a.dloss ? a.dloss[row] : 1.f) : 0.f;
@@ -199,35 +299,32 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
       } else if (MODE == kGrad) {
         w = 0.f;
       }
-      prefetch_bias_l1(a.bias, a.c0 + nbase, 128, a.V, lane);
+      if constexpr (BIAS) {  // loaded while the accumulator is still being filled
+        float4 b;
+        const int j = nbase + lane * 4;
+        b.x = j < a.n ? __ldg(a.bias + a.c0 + j) : 0.f;
+        b.y = j + 1 < a.n ? __ldg(a.bias + a.c0 + j + 1) : 0.f;
+        b.z = j + 2 < a.n ? __ldg(a.bias + a.c0 + j + 2) : 0.f;
+        b.w = j + 3 < a.n ? __ldg(a.bias + a.c0 + j + 3) : 0.f;
+        *reinterpret_cast<float4*>(bias_s + lane * 4) = b;
+        __syncwarp();
+      }
       if (!mbar_wait(&accf_bar[buf], (use >> 1) & 1, wc)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + buf * HD_BN + half * 128;
       float m = -INFINITY, s = 0.f;
+      // 32 columns at a time; the next 32 are on their way from TMEM meanwhile
+      uint32_t r[32];
+      tmem_ld32(taddr, r);
 #pragma unroll 1
       for (int c = 0; c < 128; c += 32) {
-        uint32_t r[32];
-        tmem_ld32(taddr + c, r);
-        const int n0 = nbase + c;          // column within the piece
-        const int j0 = a.c0 + n0;          // vocabulary id of column 0 of this chunk
+        tmem_ld_wait();
         float z[32];
-        if (a.bias) {
 #pragma unroll
-          for (int j8 = 0; j8 < 32; j8 += 8) {
-            float b8[8];
-            load_bias8(a.bias, j0 + j8, a.V, b8);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) z[j8 + i] = b8[i];
-          }
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) z[j] += __uint_as_float(r[j]);
-        } else {
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(r[j]);
-        }
-        if (c == 96) {  // this warp's last read of the accumulator
+        for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(r[j]);
+        if (c < 96) {
+          tmem_ld32(taddr + c + 32, r);
+        } else {  // this warp's last read of the accumulator
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -237,71 +334,34 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
               mbar_arrive_remote(&acce_bar[buf], 0);
           }
         }
-        if (n0 >= a.n) continue;  // uniform: nothing of the piece in this chunk
-        if constexpr (MODE == kStats) {
-          if (n0 + 32 > a.n) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (n0 + j >= a.n) z[j] = -INFINITY;
-          }
-          while (__any_sync(0xffffffffu, (unsigned)tg.nid - (unsigned)j0 < 32u)) {
-            const int at = (int)((unsigned)tg.nid - (unsigned)j0);
-            float v = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v = at == j ? z[j] : v;
-            if ((unsigned)at < 32u) {
-              a.zs[(size_t)row * a.K + tg.k] = v;
-              tg.next();
-            }
-          }
-          float cm = max3f(z[0], z[1], z[2]);
-#pragma unroll
-          for (int j = 3; j < 31; j += 2) cm = max3f(cm, z[j], z[j + 1]);
-          cm = fmaxf(cm, z[31]);
-          const float mn = fmaxf(m, cm);
-          const float base = mn == -INFINITY ? 0.f : mn;
-          float2 s0 = make_float2(s * ex2((m - base) * a.k), 0.f), s1 = make_float2(0.f, 0.f);
+        const int n0 = nbase + c;   // column within the piece
+        const int j0 = a.c0 + n0;   // vocabulary id of column 0
+        if (n0 >= a.n) continue;    // uniform: nothing of the piece in this chunk
+        if constexpr (BIAS) {
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
-            // subtract before scaling: exact for equal logits of any size
-            const float2 x = fsubmul2(z[j], z[j + 1], base, base, a.k, a.k);
-            const float2 y = fsubmul2(z[j + 2], z[j + 3], base, base, a.k, a.k);
-            s0 = fadd2(s0, ex2(x.x), ex2(x.y));
-            s1 = fadd2(s1, ex2(y.x), ex2(y.y));
+            const float4 b = *reinterpret_cast<const float4*>(bias_s + c + j);
+            z[j] += b.x;
+            z[j + 1] += b.y;
+            z[j + 2] += b.z;
+            z[j + 3] += b.w;
           }
-          s = (s0.x + s0.y) + (s1.x + s1.y);
-          m = mn;
+        }
+        if constexpr (MODE == kStats) {
+          stats32(z, n0, j0, row, a, tg, m, s);
         } else {
-          // G: a row without a target is exactly zero, whatever its logits hold
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float2 x = ffma2(z[j], z[j + 1], a.inv_t, -lse);
-            z[j] = ex2(x.x * kLog2e) * w;
-            z[j + 1] = ex2(x.y * kLog2e) * w;
-          }
-          if (w == 0.f) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) z[j] = 0.f;
-          }
-          while (__any_sync(0xffffffffu, (unsigned)tg.nid - (unsigned)j0 < 32u)) {
-            const int at = (int)((unsigned)tg.nid - (unsigned)j0);
-            const bool hit = (unsigned)at < 32u;
-            const float qw = hit ? (tg.qs ? tg.qs[tg.k] : 1.f) * w : 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) z[j] -= at == j ? qw : 0.f;
-            if (hit) tg.next();
-          }
-          const int hb = (c & 32) ? 4 : 0;  // 16-byte units of this half of the 64-column box
-          if (!(c & 32)) {
+          grad32(z, j0, a, tg, w, lse);
+          // 64 columns to a box; a half past the piece is not stored
+          if (!(c & 32)) {  // the box staged before has left
             if (lane == 0 && issued) bulk_wait_read0();
             __syncwarp();
           }
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            *reinterpret_cast<uint4*>(st + lane * 128 + (((u + hb) ^ (lane & 7)) << 4)) =
+            *reinterpret_cast<uint4*>(st + lane * 128 + (((u + (c >> 3 & 4)) ^ (lane & 7)) << 4)) =
                 make_uint4(pack_bf16x2(z[8 * u], z[8 * u + 1]), pack_bf16x2(z[8 * u + 2], z[8 * u + 3]),
                            pack_bf16x2(z[8 * u + 4], z[8 * u + 5]), pack_bf16x2(z[8 * u + 6], z[8 * u + 7]));
-          if ((c & 32) || n0 + 32 >= a.n) {  // box complete (or its second half lies past the piece)
+          if ((c & 32) || n0 + 32 >= a.n) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
@@ -311,18 +371,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
             ++issued;
           }
           if (a.dbp) {
-            // Column sums over the warp's 32 rows: 32 x 32 values, each step
-            // exchanging half of what is left with the lane 16, 8, ... away;
-            // lane j ends with column j (31 shuffles instead of 160).
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-              const bool up = lane & o;
-#pragma unroll
-              for (int j = 0; j < o; ++j) {
-                const float mine = up ? z[j + o] : z[j], give = up ? z[j] : z[j + o];
-                z[j] = mine + __shfl_xor_sync(0xffffffffu, give, o);
-              }
-            }
+            column_sums(z, lane);
             if (row0 < a.R && n0 + lane < a.n) a.dbp[(size_t)(row0 >> 5) * a.n + n0 + lane] = z[0];
           }
         }
@@ -358,11 +407,16 @@ cudaError_t head_logits_tc(HeadTcArgs a, const void* H, int ldh, const void* W, 
   a.tiles_m = (a.R + 2 * HD_BM - 1) / (2 * HD_BM);
   a.tiles_n = (a.n + HD_BN - 1) / HD_BN;
   const int pairs = (int)std::min<long long>((long long)a.tiles_m * a.tiles_n, num_sms() / 2);
-  auto kern = grad ? head_logits_kernel<kGrad> : head_logits_kernel<kStats>;
-  static std::atomic<unsigned long long> done[2];
-  const cudaError_t e = allow_smem(kern, HD_SMEM, done[grad]);
-  if (e != cudaSuccess) return e;
-  return launch_dependent(kern, 2 * pairs, HD_THREADS, HD_SMEM, 2, s, mh, mw, mg, a);
+  auto run = [&](auto kern, int smem, std::atomic<unsigned long long>& done) {
+    const cudaError_t e = allow_smem(kern, smem, done);
+    return e != cudaSuccess ? e : launch_dependent(kern, 2 * pairs, HD_THREADS, smem, 2, s, mh, mw, mg, a);
+  };
+  static std::atomic<unsigned long long> done[4];
+  if (grad)
+    return a.bias ? run(head_logits_kernel<kGrad, true>, HdCfg<kGrad, true>::SMEM, done[0])
+                  : run(head_logits_kernel<kGrad, false>, HdCfg<kGrad, false>::SMEM, done[1]);
+  return a.bias ? run(head_logits_kernel<kStats, true>, HdCfg<kStats, true>::SMEM, done[2])
+                : run(head_logits_kernel<kStats, false>, HdCfg<kStats, false>::SMEM, done[3]);
 }
 
 }  // namespace dgx

@@ -375,9 +375,9 @@ dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s) {
   t.n = a.V;
   cudaError_t e = target_lists(a, c, t, s);
   if (e == cudaSuccess)
-    e = small ? head_small(t, a.H, a.ldh, a.W, a.ldw, small, s)
+    e = small ? head_small(t, a.H, a.ldh, a.W, a.ldw, small, a.loss, a.lse, s)
               : head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, false, nullptr, 0, s);
-  if (e == cudaSuccess) {
+  if (e == cudaSuccess && small != 1) {
     // few slots: few warps, so that many rows do not pay for idle ones
     const bool wide = slots > 32;
     e = launch_dependent(wide ? head_finish_kernel<32> : head_finish_kernel<4>, (a.R + 31) / 32, wide ? 1024 : 128, 0, 1,

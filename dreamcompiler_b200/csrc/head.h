@@ -42,7 +42,7 @@ struct HeadArgs {
 // [c0, c0 + n) of the vocabulary, c0 a multiple of 256.
 struct HeadTcArgs {
   int R, V, d, K, c0, n;
-  int tiles_m, tiles_n;     // filled by the launcher
+  int tiles_m, tiles_n, group_m;  // filled by the launcher
   float inv_t, k;           // 1 / T, log2(e) / T
   const float* bias;        // [V] or null
   const int* sid;           // [R][K] target ids, ascending when K > 1
@@ -60,11 +60,12 @@ struct HeadTcArgs {
 cudaError_t head_logits_tc(HeadTcArgs a, const void* H, int ldh, const void* W, int ldw, bool grad, void* g, int ldg,
                            cudaStream_t s);
 
-// The forward's statistics for up to 32 rows and a hard target (head_small.cu):
+// The forward's statistics for up to 16 rows and a hard target (head_small.cu):
 // part [slots][R] and zs [R], with slots = head_small_slots() (0: not for these
-// sizes).
+// sizes; 1: loss and lse are written at once and part is not).
 int head_small_slots(int R, int V, int d);
-cudaError_t head_small(const HeadTcArgs& a, const void* H, int ldh, const void* W, int ldw, int slots, cudaStream_t s);
+cudaError_t head_small(const HeadTcArgs& a, const void* H, int ldh, const void* W, int ldw, int slots, float* loss,
+                       float* lse, cudaStream_t s);
 
 // Both gradient products of one piece (head_grads.cu). out[0] is dH [R][ld],
 // out[1] dW [n][ld]; with splits > 1 the output is fp32 partial sums

@@ -1,8 +1,8 @@
 // Forward of the vocabulary head for a few rows (a decoded token, a short
-// prompt): the logits of R <= 32 rows against every row of W, with a hard
+// prompt): the logits of R <= 16 rows against every row of W, with a hard
 // target. What counts is the stream of W (V x d bf16, read once); the products
-// are a thin tensor-core contraction on warp-level MMAs, 16 rows of W by 8 (or
-// 16, 32) rows of H, whose operand fragments the lanes load straight from
+// are a thin tensor-core contraction on warp-level MMAs, 16 rows of W by 8 or
+// 16 rows of H, whose operand fragments the lanes load straight from
 // global memory: a lane's 16 bytes of a W row are four consecutive k pairs, and
 // H is laid out in shared memory in the same order (the order of a sum's terms
 // is free), so nothing is staged or transposed.
@@ -58,14 +58,16 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 }
 
 // NT: groups of 8 rows of H. part[block][R] gets the statistics of the block's
-// columns, zs[r] the target's logit.
+// columns, zs[r] the target's logit; a single block holds all columns and writes
+// loss and lse itself.
 template <int NT>
 __global__ void __launch_bounds__(kWarps * 32) head_small_kernel(const __nv_bfloat16* __restrict__ H, int ldh,
                                                                  const __nv_bfloat16* __restrict__ W, int ldw,
                                                                  const float* __restrict__ bias,
                                                                  const int* __restrict__ target, int R, int V, int d,
-                                                                 float* __restrict__ zs, float2* __restrict__ part) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+                                                                 float* __restrict__ zs, float2* __restrict__ part,
+                                                                 float* __restrict__ loss, float* __restrict__ lse) {
+  if (gridDim.x > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the finish kernel follows
   extern __shared__ uint4 hs[];  // [chunks][NT][32 lanes]
   __shared__ float2 ms[kWarps][NT * 8];
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -146,7 +148,15 @@ __global__ void __launch_bounds__(kWarps * 32) head_small_kernel(const __nv_bflo
   if (threadIdx.x < R) {
     float mm = ms[0][threadIdx.x].x, ss = ms[0][threadIdx.x].y;
     for (int i = 1; i < kWarps; ++i) join(mm, ss, ms[i][threadIdx.x].x, ms[i][threadIdx.x].y);
-    part[(size_t)blockIdx.x * R + threadIdx.x] = make_float2(mm, ss);
+    if (gridDim.x > 1) {
+      part[(size_t)blockIdx.x * R + threadIdx.x] = make_float2(mm, ss);
+    } else {
+      const int id = target[threadIdx.x];
+      const float base = mm == -INFINITY ? 0.f : mm, log_s = logf(ss);
+      lse[threadIdx.x] = base + log_s;
+      // zs[row] was written by this block before the barrier
+      loss[threadIdx.x] = id >= 0 && id < V ? log_s - (__ldcg(zs + threadIdx.x) - base) : 0.f;
+    }
   }
 }
 
@@ -162,13 +172,14 @@ int head_small_slots(int R, int V, int d) {
   return std::min((tiles + kWarps - 1) / kWarps, 2 * num_sms());
 }
 
-cudaError_t head_small(const HeadTcArgs& a, const void* H, int ldh, const void* W, int ldw, int slots, cudaStream_t s) {
+cudaError_t head_small(const HeadTcArgs& a, const void* H, int ldh, const void* W, int ldw, int slots, float* loss,
+                       float* lse, cudaStream_t s) {
   const int smem = small_smem(a.R, a.d);
   auto run = [&](auto kern, std::atomic<unsigned long long>& done) {
     const cudaError_t e = allow_smem(kern, 96 * 1024, done);
     if (e != cudaSuccess) return e;
     return launch_dependent(kern, slots, kWarps * 32, smem, 1, s, (const __nv_bfloat16*)H, ldh, (const __nv_bfloat16*)W,
-                            ldw, a.bias, a.sid, a.R, a.V, a.d, a.zs, a.part);
+                            ldw, a.bias, a.sid, a.R, a.V, a.d, a.zs, a.part, loss, lse);
   };
   static std::atomic<unsigned long long> done[2];
   return a.R <= 8 ? run(head_small_kernel<1>, done[0]) : run(head_small_kernel<2>, done[1]);

@@ -250,22 +250,26 @@ def _ws(workspace: Optional[torch.Tensor]):
 
 
 def _head_check(H, W, bias, rows32, rowsf):
-    """Shapes and types shared by the vocabulary-head wrappers; returns (R, V, d)."""
-    assert H.is_cuda and H.dtype == torch.bfloat16 and H.dim() == 2 and H.stride(1) == 1, "H: [R, d] bf16 CUDA rows"
-    assert W.device == H.device and W.dtype == torch.bfloat16 and W.dim() == 2 and W.stride(1) == 1, "W: [V, d] bf16 rows"
-    (R, d), V = H.shape, W.shape[0]
-    assert W.shape[1] == d, f"H has {d} columns, W {W.shape[1]}"
+    """Shapes and types shared by the vocabulary-head wrappers; returns (R, V,
+    d) and the row pitches of H and W. Each attribute of a tensor is asked for
+    once: for a few rows these checks weigh as much as the kernels."""
+    dev = H.get_device()
+    assert dev >= 0 and H.dtype is torch.bfloat16 and H.dim() == 2, "H: [R, d] bf16 CUDA rows"
+    assert W.get_device() == dev and W.dtype is torch.bfloat16 and W.dim() == 2, "W: [V, d] bf16 rows on H's device"
+    (R, d), (V, dw), (ldh, sh), (ldw, sw) = H.shape, W.shape, H.stride(), W.stride()
+    assert dw == d, f"H has {d} columns, W {dw}"
+    assert (sh == 1 or d == 1) and (sw == 1 or d == 1), "the columns of H and W must be contiguous"
     if bias is not None:
-        assert bias.device == H.device and bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == V
-    assert rows32.device == H.device and rows32.dtype == torch.int32 and rows32.is_contiguous() and rows32.shape[0] == R
+        assert bias.get_device() == dev and bias.dtype is torch.float32 and bias.is_contiguous() and bias.numel() == V
+    assert rows32.get_device() == dev and rows32.dtype is torch.int32 and rows32.is_contiguous() and rows32.shape[0] == R
     for t in rowsf:
         if t is not None:
-            assert t.device == H.device and t.dtype == torch.float32 and t.is_contiguous() and t.shape[0] == R
-    return R, V, d
+            assert t.get_device() == dev and t.dtype is torch.float32 and t.is_contiguous() and t.shape[0] == R
+    # torch reports any stride for a single row
+    return R, V, d, ldh if R > 1 else (d + 7) // 8 * 8, ldw if V > 1 else (d + 7) // 8 * 8
 
 
 def _pitch(t: torch.Tensor) -> int:
-    """Row pitch in elements. torch reports any stride for a single row."""
     return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
 
 
@@ -289,14 +293,14 @@ def linear_nll_fwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, *, bi
     int32 (outside [0, V): no target, loss 0). Returns (loss [R], lse [R]), the
     row log-sum-exp being what linear_nll_bwd needs; `mean` (one fp32 element)
     receives sum(loss) / R."""
-    R, V, d = _head_check(H, W, bias, target, (loss, lse))
+    R, V, d, ldh, ldw = _head_check(H, W, bias, target, (loss, lse))
     assert target.dim() == 1
     if loss is None:
         loss = torch.empty(R, device=H.device, dtype=torch.float32)
     if lse is None:
         lse = torch.empty(R, device=H.device, dtype=torch.float32)
     ws, wsb = _ws(workspace)
-    L.call("dgx_linear_nll_fwd", H.data_ptr(), _pitch(H), W.data_ptr(), _pitch(W), _ptr(bias), target.data_ptr(), R, V,
+    L.call("dgx_linear_nll_fwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), target.data_ptr(), R, V,
            d, loss.data_ptr(), lse.data_ptr(), _ptr(mean), ws, wsb, _stream(H))
     return loss, lse
 
@@ -310,10 +314,10 @@ def linear_nll_bwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, lse: 
     (dH [R, d], dW [V, d], db [V] fp32); those not in `need` (and db without a
     bias) are None. dH and dW are new bf16 tensors unless given (bf16 or fp32);
     accumulate adds to the given fp32 dW and db."""
-    R, V, d = _head_check(H, W, bias, target, (lse, dloss))
+    R, V, d, ldh, ldw = _head_check(H, W, bias, target, (lse, dloss))
     dH, dW, db = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate)
     ws, wsb = _ws(workspace)
-    L.call("dgx_linear_nll_bwd", H.data_ptr(), _pitch(H), W.data_ptr(), _pitch(W), _ptr(bias), target.data_ptr(),
+    L.call("dgx_linear_nll_bwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), target.data_ptr(),
            lse.data_ptr(), _ptr(dloss), float(scale), R, V, d, *_grad_args(dH), *_grad_args(dW), _ptr(db),
            int(accumulate), ws, wsb, _stream(H))
     return dH, dW, db
@@ -345,14 +349,14 @@ def linear_distill_fwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teac
     against a teacher's K largest logits per row: idx [R, K] int32 vocabulary
     ids (outside [0, V): absent), teacher [R, K] fp32. Returns (loss [R],
     lse [R]) with lse the log-sum-exp of the student's logits / T."""
-    R, V, d = _head_check(H, W, bias, idx, (teacher, loss, lse))
+    R, V, d, ldh, ldw = _head_check(H, W, bias, idx, (teacher, loss, lse))
     assert idx.dim() == 2 and teacher.shape == idx.shape
     if loss is None:
         loss = torch.empty(R, device=H.device, dtype=torch.float32)
     if lse is None:
         lse = torch.empty(R, device=H.device, dtype=torch.float32)
     ws, wsb = _ws(workspace)
-    L.call("dgx_linear_distill_fwd", H.data_ptr(), _pitch(H), W.data_ptr(), _pitch(W), _ptr(bias), idx.data_ptr(),
+    L.call("dgx_linear_distill_fwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), idx.data_ptr(),
            teacher.data_ptr(), idx.shape[1], float(temperature), R, V, d, loss.data_ptr(), lse.data_ptr(), _ptr(mean),
            ws, wsb, _stream(H))
     return loss, lse
@@ -364,18 +368,17 @@ def linear_distill_bwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teac
                        dW: Optional[torch.Tensor] = None, db: Optional[torch.Tensor] = None,
                        need=("dH", "dW", "db"), accumulate: bool = False, workspace: Optional[torch.Tensor] = None):
     """Gradients of sum_r scale * dloss[r] * loss[r]; arguments and results as linear_nll_bwd."""
-    R, V, d = _head_check(H, W, bias, idx, (teacher, lse, dloss))
+    R, V, d, ldh, ldw = _head_check(H, W, bias, idx, (teacher, lse, dloss))
     assert idx.dim() == 2 and teacher.shape == idx.shape
     dH, dW, db = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate)
     ws, wsb = _ws(workspace)
-    L.call("dgx_linear_distill_bwd", H.data_ptr(), _pitch(H), W.data_ptr(), _pitch(W), _ptr(bias), idx.data_ptr(),
+    L.call("dgx_linear_distill_bwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), idx.data_ptr(),
            teacher.data_ptr(), idx.shape[1], float(temperature), lse.data_ptr(), _ptr(dloss), float(scale), R, V, d,
            *_grad_args(dH), *_grad_args(dW), _ptr(db), int(accumulate), ws, wsb, _stream(H))
     return dH, dW, db
 
 
-def _row_ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+_ROW_DT = {torch.float32: L.DGX_F32, torch.bfloat16: L.DGX_BF16}
 
 
 def embed_fwd(tok: torch.Tensor, W: torch.Tensor, *, scale: float = 1.0, pos: Optional[torch.Tensor] = None,
@@ -383,17 +386,22 @@ def embed_fwd(tok: torch.Tensor, W: torch.Tensor, *, scale: float = 1.0, pos: Op
     """x[i] = scale * W[tok[i]] (+ pos[i % len(pos)]): tok int32 of any shape
     (taken flat), W [V, d] fp32 or bf16, pos [S, d] fp32, out [n, d] fp32 or
     bf16 (W's type by default). An id outside [0, V) gives a zero row (+ pos)."""
-    assert W.is_cuda and W.dtype in (torch.float32, torch.bfloat16) and W.dim() == 2 and W.stride(1) == 1
-    assert tok.device == W.device and tok.dtype == torch.int32 and tok.is_contiguous()
-    n, (V, d) = tok.numel(), W.shape
+    dev, wt = W.get_device(), _ROW_DT.get(W.dtype)
+    assert dev >= 0 and wt is not None and W.dim() == 2, "W: [V, d] fp32 or bf16 CUDA rows"
+    assert tok.get_device() == dev and tok.dtype is torch.int32 and tok.is_contiguous(), "tok: int32 ids on W's device"
+    n, (V, d), (ldw, sw) = tok.numel(), W.shape, W.stride()
+    S = 0
     if pos is not None:
-        assert pos.device == W.device and pos.dtype == torch.float32 and pos.is_contiguous() and pos.dim() == 2 and pos.shape[1] == d
+        assert pos.get_device() == dev and pos.dtype is torch.float32 and pos.is_contiguous() and pos.dim() == 2 and pos.shape[1] == d
+        S = pos.shape[0]
     if out is None:
-        out = torch.empty(n, d, device=W.device, dtype=out_dtype or W.dtype)
-    assert out.device == W.device and out.shape == (n, d) and out.stride(1) == 1 and out.dtype in (torch.float32, torch.bfloat16)
-    L.call("dgx_embed_fwd", tok.data_ptr(), W.data_ptr(), _DT[W.dtype], _row_ld(W), _ptr(pos),
-           0 if pos is None else pos.shape[0], float(scale), out.data_ptr(), _DT[out.dtype], _row_ld(out), n, d, V,
-           _stream(W))
+        out, xt, ldx = torch.empty(n, d, device=W.device, dtype=out_dtype or W.dtype), _ROW_DT[out_dtype or W.dtype], d
+    else:
+        xt, (ldx, sx) = _ROW_DT.get(out.dtype), out.stride()
+        assert out.get_device() == dev and out.shape == (n, d) and (sx == 1 or d == 1) and xt is not None
+    assert sw == 1 or d == 1, "the columns of W must be contiguous"
+    L.call("dgx_embed_fwd", tok.data_ptr(), W.data_ptr(), wt, ldw if V > 1 else d, None if pos is None else pos.data_ptr(),
+           S, float(scale), out.data_ptr(), xt, ldx if n > 1 else d, n, d, V, _stream(W))
     return out
 
 
@@ -407,16 +415,20 @@ def embed_bwd(tok: torch.Tensor, dx: torch.Tensor, V: int, *, scale: float = 1.0
     """dW[t] = scale * sum of dx[i] over tok[i] == t, in ascending i: dx [n, d]
     fp32 or bf16, dW [V, d] of out_dtype (or the given `out`; accumulate adds
     to an fp32 one). The same bits on every run."""
-    assert dx.is_cuda and dx.dtype in (torch.float32, torch.bfloat16) and dx.dim() == 2 and dx.stride(1) == 1
-    assert tok.device == dx.device and tok.dtype == torch.int32 and tok.is_contiguous() and tok.numel() == dx.shape[0]
-    n, d = dx.shape
+    dev, gt = dx.get_device(), _ROW_DT.get(dx.dtype)
+    assert dev >= 0 and gt is not None and dx.dim() == 2, "dx: [n, d] fp32 or bf16 CUDA rows"
+    (n, d), (lddx, sg) = dx.shape, dx.stride()
+    assert sg == 1 or d == 1, "the columns of dx must be contiguous"
+    assert tok.get_device() == dev and tok.dtype is torch.int32 and tok.is_contiguous() and tok.numel() == n, \
+        "tok: one int32 id per row of dx"
     if out is None:
         assert not accumulate, "accumulate needs the tensor to add to"
         out = torch.empty(V, d, device=dx.device, dtype=out_dtype)
-    assert out.device == dx.device and out.shape == (V, d) and out.stride(1) == 1 and out.dtype in (torch.float32, torch.bfloat16)
+    wt, (lddw, so) = _ROW_DT.get(out.dtype), out.stride()
+    assert out.get_device() == dev and out.shape == (V, d) and (so == 1 or d == 1) and wt is not None
     ws, wsb = _ws(workspace)
-    L.call("dgx_embed_bwd", tok.data_ptr(), dx.data_ptr(), _DT[dx.dtype], _row_ld(dx), float(scale), out.data_ptr(),
-           _DT[out.dtype], _row_ld(out), n, d, V, int(accumulate), ws, wsb, _stream(dx))
+    L.call("dgx_embed_bwd", tok.data_ptr(), dx.data_ptr(), gt, lddx if n > 1 else d, float(scale), out.data_ptr(), wt,
+           lddw if V > 1 else d, n, d, V, int(accumulate), ws, wsb, _stream(dx))
     return out
 
 

@@ -121,6 +121,7 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const int* __restrict__ 
                                                         const float* __restrict__ P, int S, float scale,
                                                         TX* __restrict__ x, int ldx, int n, int d, int V, int slabs) {
   constexpr int kRows = fwd_rows<TW, VEC>();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const unsigned item = blockIdx.x * 8u + (threadIdx.x >> 5);
   const unsigned group = item / (unsigned)slabs;
@@ -171,6 +172,9 @@ struct SortArgs {
 };
 
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortArgs a) {
+  // in this order: the zeroing kernel does not wait for anything itself, so it
+  // may start only when all that came before this call is done
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ int hist[];              // [kSortWarps][bins]
   cg::cluster_group cluster = cg::this_cluster();
@@ -630,19 +634,7 @@ cudaError_t launch_sort(const SortArgs& a, cudaStream_t s) {
   const int wide = wide_cluster();
   // up to 4096 tokens one CTA sorts without leaving its SM
   const int cluster = a.n <= 4096 ? 1 : a.n <= 8192 ? 8 : wide;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(cluster);
-  cfg.blockDim = dim3(kSortThreads);
-  cfg.dynamicSmemBytes = kSortWarps * 4 << a.bits;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, embed_sort_kernel, a);
+  return launch_dependent(embed_sort_kernel, cluster, kSortThreads, kSortWarps * 4 << a.bits, cluster, s, a);
 }
 
 cudaError_t launch_zero(const ZeroArgs& a, cudaStream_t s) {
@@ -680,18 +672,20 @@ dgx_status dgx_embed_fwd(const int* tok, const void* W, dgx_dtype w_type, int ld
   const int rows = vec && w_type == DGX_BF16 ? fwd_rows<__nv_bfloat16, true>() : fwd_rows<float, true>();
   const long long items = ((long long)n + rows - 1) / rows * slabs;
   if (items > 0x7fffffffll) return set_error(DGX_EINVAL, "dgx_embed_fwd: n=%d d=%d too large", n, d);
+  cudaError_t e = cudaSuccess;
   auto run = [&](auto* w, auto* o) {
     using TW = std::remove_const_t<std::remove_pointer_t<decltype(w)>>;
     using TX = std::remove_pointer_t<decltype(o)>;
     auto k = vec ? (P ? embed_fwd_kernel<TW, TX, true, true> : embed_fwd_kernel<TW, TX, true, false>)
                  : (P ? embed_fwd_kernel<TW, TX, false, true> : embed_fwd_kernel<TW, TX, false, false>);
-    k<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(tok, w, ldw, P, P ? S : 1, scale, o, ldx, n, d, V, slabs);
+    e = launch_dependent(k, (unsigned)((items + 7) / 8), 256, 0, 1, s, tok, w, ldw, P, P ? S : 1, scale, o, ldx, n, d, V,
+                         slabs);
   };
   if (w_type == DGX_F32 && x_type == DGX_F32) run((const float*)W, (float*)x);
   else if (w_type == DGX_F32) run((const float*)W, (__nv_bfloat16*)x);
   else if (x_type == DGX_F32) run((const __nv_bfloat16*)W, (float*)x);
   else run((const __nv_bfloat16*)W, (__nv_bfloat16*)x);
-  return cuda_status(cudaGetLastError(), "dgx_embed_fwd");
+  return cuda_status(e, "dgx_embed_fwd");
 }
 
 size_t dgx_embed_bwd_workspace_size(int n, int d, int V) {

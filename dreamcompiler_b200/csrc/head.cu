@@ -415,7 +415,7 @@ dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
     e = head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, true, g, p.pc, s);
     if (e != cudaSuccess) return cuda_status(e, "head backward");
     if (a.db) {
-      e = launch_dependent(head_db_kernel, (n + 31) / 32, 256, 0, 1, s, dbp, p.slabs, n, a.scale, a.accumulate,
+      e = launch_dependent(head_db_kernel, (n + 31) / 32, 256, 0, 1, s, dbp, p.slabs, n, a.scale, a.add_w,
                            a.db + c0);
       if (e != cudaSuccess) return cuda_status(e, "head backward");
     }
@@ -431,13 +431,13 @@ dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
     m.d = a.d;
     m.err = a.err;
     void* dw_out = a.dW ? (char*)a.dW + (size_t)c0 * a.lddw * (a.dw_bf16 ? 2 : 4) : nullptr;
-    if (a.dH) m.out[0] = dh ? GradOut{dh, 0, c0 > 0, p.dp, p.sp.dh, 1.f} : GradOut{a.dH, a.dh_bf16, 0, a.lddh, 1, a.scale};
-    if (a.dW) m.out[1] = dw ? GradOut{dw, 0, 0, p.dp, p.sp.dw, 1.f} : GradOut{dw_out, a.dw_bf16, a.accumulate, a.lddw, 1, a.scale};
+    if (a.dH) m.out[0] = dh ? GradOut{dh, 0, c0 > 0, p.dp, p.sp.dh, 1.f} : GradOut{a.dH, a.dh_bf16, a.add_h, a.lddh, 1, a.scale};
+    if (a.dW) m.out[1] = dw ? GradOut{dw, 0, 0, p.dp, p.sp.dw, 1.f} : GradOut{dw_out, a.dw_bf16, a.add_w, a.lddw, 1, a.scale};
     e = head_grads_tc(m, s);
-    if (e == cudaSuccess && a.dW && dw) e = launch_out(dw, p.sp.dw, n, a, p.dp, a.dw_bf16, a.accumulate, dw_out, a.lddw, s);
+    if (e == cudaSuccess && a.dW && dw) e = launch_out(dw, p.sp.dw, n, a, p.dp, a.dw_bf16, a.add_w, dw_out, a.lddw, s);
     if (e != cudaSuccess) return cuda_status(e, "head backward");
   }
-  if (a.dH && dh) e = launch_out(dh, p.sp.dh, a.R, a, p.dp, a.dh_bf16, 0, a.dH, a.lddh, s);
+  if (a.dH && dh) e = launch_out(dh, p.sp.dh, a.R, a, p.dp, a.dh_bf16, a.add_h, a.dH, a.lddh, s);
   return cuda_status(e, "head backward");
 }
 

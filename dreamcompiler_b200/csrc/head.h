@@ -34,7 +34,7 @@ struct HeadArgs {
   void* dW;            // [V][lddw] or null
   float* db;           // [V] or null
   int dh_bf16, lddh, dw_bf16, lddw;
-  int accumulate;      // dW (fp32) and db are added to
+  int add_w, add_h;    // dW (fp32) and db, dH (fp32) are added to
   uint32_t* err;
 };
 

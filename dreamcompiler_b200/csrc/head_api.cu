@@ -50,7 +50,7 @@ dgx_status run_fwd(const char* op, HeadArgs& a, void* ws, size_t ws_bytes, cudaS
   return head_fwd(a, ws, s);
 }
 
-dgx_status run_bwd(const char* op, HeadArgs& a, int dh_type, int dw_type, void* ws, size_t ws_bytes, cudaStream_t s) {
+dgx_status run_bwd(const char* op, HeadArgs& a, int dh_type, int dw_type, int accumulate, void* ws, size_t ws_bytes, cudaStream_t s) {
   dgx_status st = head_check(op, a.H, a.ldh, a.W, a.ldw, a.R, a.V, a.d, a.K);
   if (st != DGX_OK) return st;
   if (a.dH && dh_type != DGX_F32 && dh_type != DGX_BF16) return set_error(DGX_EINVAL, "%s: dH type %d", op, dh_type);
@@ -62,13 +62,16 @@ dgx_status run_bwd(const char* op, HeadArgs& a, int dh_type, int dw_type, void* 
     return set_error(DGX_EINVAL, "%s: dH needs 16-byte aligned rows of at least d=%d elements (lddh=%d)", op, a.d, a.lddh);
   if (a.dW && (a.lddw < a.d || a.lddw % wq || ((uintptr_t)a.dW & 15)))
     return set_error(DGX_EINVAL, "%s: dW needs 16-byte aligned rows of at least d=%d elements (lddw=%d)", op, a.d, a.lddw);
-  if (a.accumulate && a.dW && a.dw_bf16)
-    return set_error(DGX_EUNSUPPORTED, "%s: accumulate needs an fp32 dW", op);
+  if (accumulate & ~(DGX_ACC_W | DGX_ACC_H)) return set_error(DGX_EINVAL, "%s: accumulate %d", op, accumulate);
+  a.add_w = (accumulate & DGX_ACC_W) != 0;
+  a.add_h = (accumulate & DGX_ACC_H) != 0;
+  if ((a.add_w && a.dW && a.dw_bf16) || (a.add_h && a.dH && a.dh_bf16))
+    return set_error(DGX_EUNSUPPORTED, "%s: accumulate needs an fp32 %s", op, a.add_w && a.dw_bf16 ? "dW" : "dH");
   if (a.R == 0) {  // a sum over no rows
     cudaError_t e = cudaSuccess;
-    if (!a.accumulate && a.dW)
+    if (!a.add_w && a.dW)
       e = cudaMemset2DAsync(a.dW, (size_t)a.lddw * (a.dw_bf16 ? 2 : 4), 0, (size_t)a.d * (a.dw_bf16 ? 2 : 4), a.V, s);
-    if (e == cudaSuccess && !a.accumulate && a.db) e = cudaMemsetAsync(a.db, 0, (size_t)a.V * sizeof(float), s);
+    if (e == cudaSuccess && !a.add_w && a.db) e = cudaMemsetAsync(a.db, 0, (size_t)a.V * sizeof(float), s);
     return cuda_status(e, op);
   }
   if (!a.idx || !a.lse) return set_error(DGX_EINVAL, "%s: null pointer", op);
@@ -146,8 +149,7 @@ dgx_status dgx_linear_nll_bwd(const void* H, int ldh, const void* W, int ldw, co
   a.dW = dW;
   a.lddw = lddw;
   a.db = db;
-  a.accumulate = accumulate ? 1 : 0;
-  return run_bwd("dgx_linear_nll_bwd", a, dh_type, dw_type, workspace, workspace_bytes, (cudaStream_t)stream);
+  return run_bwd("dgx_linear_nll_bwd", a, dh_type, dw_type, accumulate, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 dgx_status dgx_linear_distill_fwd(const void* H, int ldh, const void* W, int ldw, const float* bias, const int* idx,
@@ -209,8 +211,7 @@ dgx_status dgx_linear_distill_bwd(const void* H, int ldh, const void* W, int ldw
   a.dW = dW;
   a.lddw = lddw;
   a.db = db;
-  a.accumulate = accumulate ? 1 : 0;
-  return run_bwd("dgx_linear_distill_bwd", a, dh_type, dw_type, workspace, workspace_bytes, (cudaStream_t)stream);
+  return run_bwd("dgx_linear_distill_bwd", a, dh_type, dw_type, accumulate, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -16,6 +16,14 @@ and its gradient) are produced in bf16 by the GEMM epilogue.
 
 All buffers are allocated up front, so one `step` can be captured in a CUDA
 graph and replayed (the AdamW step count lives on the device).
+
+With ``fused_vocab=True`` the two ends of the step that are as large as the
+vocabulary run on the operators made for it: the embedding with a scale and its
+gradient summed in token order (dgx_embed_fwd / dgx_embed_bwd), and the output
+layer, softmax and loss in one operator that keeps no logits
+(dgx_linear_nll_fwd / _bwd). ``teacher_k`` > 0 adds distillation from a
+teacher's largest logits (dgx_linear_distill_fwd / _bwd; ``set_teacher``): the
+loss becomes (1 - a) nll + a distillation with a = ``teacher_weight``.
 """
 from __future__ import annotations
 
@@ -25,7 +33,9 @@ from typing import Dict
 import torch
 
 from . import _lib as L
-from .ops import _stream, flash_bwd_workspace_size, gemm
+from .ops import (_stream, embed_bwd, embed_bwd_workspace_size, embed_fwd, flash_bwd_workspace_size, gemm,
+                  linear_distill_bwd, linear_distill_fwd, linear_distill_workspace_size, linear_nll_bwd, linear_nll_fwd,
+                  linear_nll_workspace_size)
 
 
 @dataclass
@@ -40,6 +50,11 @@ class GPTConfig:
     betas: tuple = (0.9, 0.999)
     eps: float = 1e-8
     weight_decay: float = 0.01
+    fused_vocab: bool = False     # the vocabulary-sized operators instead of logits in memory
+    embed_scale: float = 1.0      # fused_vocab only
+    teacher_k: int = 0            # teacher logits per position (fused_vocab only); 0: no distillation
+    teacher_weight: float = 0.5
+    temperature: float = 1.0
 
     @property
     def head_dim(self) -> int:
@@ -119,9 +134,13 @@ class GPT:
         self.att16 = [torch.empty(R, d, device=dev, dtype=bf16) for _ in range(c.n_layer)]
         self.u16 = [torch.empty(R, 4 * d, device=dev, dtype=bf16) for _ in range(c.n_layer)]
         self.g16 = [torch.empty(R, 4 * d, device=dev, dtype=bf16) for _ in range(c.n_layer)]
-        self.logits = torch.empty(R, Vp, device=dev, dtype=f32)
-        self.dlogits = torch.empty(R, Vp, device=dev, dtype=bf16)
         self.loss = torch.zeros(1, device=dev, dtype=f32)
+        if c.fused_vocab:
+            self._alloc_vocab()
+        else:
+            assert c.teacher_k == 0 and c.embed_scale == 1.0, "distillation and the embedding scale need fused_vocab"
+            self.logits = torch.empty(R, Vp, device=dev, dtype=f32)
+            self.dlogits = torch.empty(R, Vp, device=dev, dtype=bf16)
         # ---- backward scratch
         self.dx = torch.empty(R, d, device=dev, dtype=f32)
         self.dx16 = torch.empty(R, d, device=dev, dtype=bf16)
@@ -131,6 +150,19 @@ class GPT:
         self.dqkv16 = torch.empty(R, 3 * d, device=dev, dtype=bf16)
         self.datt16 = torch.empty(R, d, device=dev, dtype=bf16)
         self.fa_ws = torch.empty(flash_bwd_workspace_size(B * H, S, hd) // 4 + 1, device=dev, dtype=f32)
+
+    def _alloc_vocab(self):
+        """Row results and one workspace for the vocabulary-sized operators
+        (they run one after the other)."""
+        c, dev, R, d, V, K = self.cfg, self.dev, self.R, self.cfg.d_model, self.cfg.vocab, self.cfg.teacher_k
+        self.row_loss, self.row_lse = (torch.empty(R, device=dev, dtype=torch.float32) for _ in range(2))
+        need = [embed_bwd_workspace_size(R, d, V)] + [linear_nll_workspace_size(R, V, d, b) for b in (False, True)]
+        if K:
+            self.teacher_idx = torch.full((R, K), -1, device=dev, dtype=torch.int32)
+            self.teacher_logits = torch.zeros(R, K, device=dev, dtype=torch.float32)
+            self.distill_loss = torch.zeros(1, device=dev, dtype=torch.float32)
+            need += [linear_distill_workspace_size(R, V, d, K, b) for b in (False, True)]
+        self.vocab_ws = torch.empty(max(need), device=dev, dtype=torch.uint8)
 
     # ------------------------------------------------------------ setup
     def _init(self, params, seed):
@@ -161,6 +193,48 @@ class GPT:
         self.tok.copy_(tok.reshape(-1), non_blocking=True)
         self.tgt.copy_(tgt.reshape(-1), non_blocking=True)
 
+    def set_teacher(self, idx: torch.Tensor, logits: torch.Tensor):
+        """The teacher's teacher_k largest logits per position: ids (outside the
+        vocabulary: absent) and values, [batch * seq_len, teacher_k]."""
+        self.teacher_idx.copy_(idx.reshape(self.teacher_idx.shape), non_blocking=True)
+        self.teacher_logits.copy_(logits.reshape(self.teacher_logits.shape), non_blocking=True)
+
+    # ------------------------------------------------------------ the vocabulary-sized ends
+    def _embed(self):
+        c, p = self.cfg, self.p
+        if c.fused_vocab:
+            embed_fwd(self.tok, p["W_tok"], scale=c.embed_scale, pos=p["P"], out=self.x[0])
+        else:
+            _c("dgx_embedding_fwd", self.tok.data_ptr(), p["W_tok"].data_ptr(), p["P"].data_ptr(),
+               self.x[0].data_ptr(), self.R, c.seq_len, c.d_model, c.vocab, _stream(self.x[0]))
+
+    def _embed_backward(self):
+        c, g, s = self.cfg, self.g, _stream(self.dx)
+        if c.fused_vocab:
+            embed_bwd(self.tok, self.dx, c.vocab, scale=c.embed_scale, out=g["W_tok"], workspace=self.vocab_ws)
+            # dP[s] = sum over the batch: column sums of dx seen as [batch][S * d]
+            _c("dgx_colsum", self.dx.data_ptr(), L.DGX_F32, g["P"].data_ptr(), c.batch, c.seq_len * c.d_model, 0, s)
+        else:
+            g["W_tok"].zero_()
+            g["P"].zero_()
+            _c("dgx_embedding_bwd", self.tok.data_ptr(), self.dx.data_ptr(), g["W_tok"].data_ptr(), g["P"].data_ptr(),
+               self.R, c.seq_len, c.d_model, c.vocab, s)
+
+    def _head_fused(self, hf):
+        """Loss, and its gradient in dh (fp32), g["Wout"] and g["bout"], without logits."""
+        c, R, V, ws = self.cfg, self.R, self.cfg.vocab, self.vocab_ws
+        W, b = self.w16["Wout"][:V], self.p["bout"][:V]
+        out = dict(bias=b, dH=self.dh, dW=self.g["Wout"][:V], db=self.g["bout"][:V], workspace=ws)
+        share = 1.0 - c.teacher_weight if c.teacher_k else 1.0
+        linear_nll_fwd(hf, W, self.tgt, bias=b, loss=self.row_loss, lse=self.row_lse, mean=self.loss, workspace=ws)
+        linear_nll_bwd(hf, W, self.tgt, self.row_lse, scale=share / R, **out)
+        if c.teacher_k:
+            t = (self.teacher_idx, self.teacher_logits)
+            linear_distill_fwd(hf, W, *t, bias=b, temperature=c.temperature, loss=self.row_loss, lse=self.row_lse,
+                               mean=self.distill_loss, workspace=ws)
+            linear_distill_bwd(hf, W, *t, self.row_lse, temperature=c.temperature, scale=c.teacher_weight / R,
+                               accumulate=True, accumulate_dH=True, **out)
+
     # ------------------------------------------------------------ step
     def forward_backward(self):
         c = self.cfg
@@ -168,8 +242,7 @@ class GPT:
         s = _stream(self.x[0])
         p, g, w = self.p, self.g, self.w16
         # ---- forward
-        _c("dgx_embedding_fwd", self.tok.data_ptr(), p["W_tok"].data_ptr(), p["P"].data_ptr(), self.x[0].data_ptr(),
-           R, S, d, V, s)
+        self._embed()
         for l in range(c.n_layer):
             x0, x1, x2 = self.x[2 * l], self.x[2 * l + 1], self.x[2 * l + 2]
             h, h2 = self.h16[2 * l], self.h16[2 * l + 1]
@@ -190,13 +263,17 @@ class GPT:
             gemm(self.g16[l], w[f"W2{l}"], transB=True, out=x2, bias=p[f"b2{l}"], beta=1.0)
         xL, hf = self.x[2 * c.n_layer], self.h16[2 * c.n_layer]
         _c("dgx_layernorm_fwd", xL.data_ptr(), hf.data_ptr(), self.mu[-1].data_ptr(), self.rs[-1].data_ptr(), R, d, s)
-        gemm(hf, w["Wout"], transB=True, out=self.logits, bias=p["bout"])
-        _c("dgx_softmax_nll", self.logits.data_ptr(), Vp, V, self.tgt.data_ptr(), R, self.loss.data_ptr(),
-           self.dlogits.data_ptr(), L.DGX_BF16, s)
-        # ---- backward
-        gemm(self.dlogits, w["Wout"], out=self.dh)                        # dhf = dlogits Wout
-        gemm(self.dlogits, hf, transA=True, out=g["Wout"])                # dWout = dlogits^T hf
-        _c("dgx_colsum", self.dlogits.data_ptr(), L.DGX_BF16, g["bout"].data_ptr(), R, Vp, 0, s)
+        # ---- head and loss, forward and backward: dh = d loss / d hf
+        if c.fused_vocab:
+            self._head_fused(hf)
+        else:
+            gemm(hf, w["Wout"], transB=True, out=self.logits, bias=p["bout"])
+            _c("dgx_softmax_nll", self.logits.data_ptr(), Vp, V, self.tgt.data_ptr(), R, self.loss.data_ptr(),
+               self.dlogits.data_ptr(), L.DGX_BF16, s)
+            gemm(self.dlogits, w["Wout"], out=self.dh)                        # dhf = dlogits Wout
+            gemm(self.dlogits, hf, transA=True, out=g["Wout"])                # dWout = dlogits^T hf
+            _c("dgx_colsum", self.dlogits.data_ptr(), L.DGX_BF16, g["bout"].data_ptr(), R, Vp, 0, s)
+        # ---- backward through the blocks
         # each layer-norm backward also leaves bf16(dx) in dx16 for the next GEMMs
         _c("dgx_layernorm_bwd_x16", xL.data_ptr(), self.mu[-1].data_ptr(), self.rs[-1].data_ptr(),
            self.dh.data_ptr(), self.dx.data_ptr(), self.dx16.data_ptr(), R, d, 0, s)
@@ -232,10 +309,7 @@ class GPT:
             else:  # the embedding backward reads dx in fp32 only
                 _c("dgx_layernorm_bwd", x0.data_ptr(), self.mu[2 * l].data_ptr(), self.rs[2 * l].data_ptr(),
                    self.dh.data_ptr(), self.dx.data_ptr(), R, d, 1, s)
-        g["W_tok"].zero_()
-        g["P"].zero_()
-        _c("dgx_embedding_bwd", self.tok.data_ptr(), self.dx.data_ptr(), g["W_tok"].data_ptr(), g["P"].data_ptr(),
-           R, S, d, V, s)
+        self._embed_backward()
         return self.loss
 
     def optimizer_step(self):

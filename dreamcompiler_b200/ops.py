@@ -308,24 +308,25 @@ def linear_nll_fwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, *, bi
 def linear_nll_bwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, *,
                    bias: Optional[torch.Tensor] = None, dloss: Optional[torch.Tensor] = None, scale: float = 1.0,
                    dH: Optional[torch.Tensor] = None, dW: Optional[torch.Tensor] = None,
-                   db: Optional[torch.Tensor] = None, need=("dH", "dW", "db"), accumulate: bool = False,
+                   db: Optional[torch.Tensor] = None, need=("dH", "dW", "db"), accumulate: bool = False, accumulate_dH: bool = False,
                    workspace: Optional[torch.Tensor] = None):
     """Gradients of sum_r scale * dloss[r] * loss[r] (dloss None: 1). Returns
     (dH [R, d], dW [V, d], db [V] fp32); those not in `need` (and db without a
     bias) are None. dH and dW are new bf16 tensors unless given (bf16 or fp32);
-    accumulate adds to the given fp32 dW and db."""
+    accumulate adds to the given fp32 dW and db, accumulate_dH to the fp32 dH."""
     R, V, d, ldh, ldw = _head_check(H, W, bias, target, (lse, dloss))
-    dH, dW, db = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate)
+    dH, dW, db = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH)
     ws, wsb = _ws(workspace)
     L.call("dgx_linear_nll_bwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), target.data_ptr(),
            lse.data_ptr(), _ptr(dloss), float(scale), R, V, d, *_grad_args(dH), *_grad_args(dW), _ptr(db),
-           int(accumulate), ws, wsb, _stream(H))
+           int(accumulate) + 2 * int(accumulate_dH), ws, wsb, _stream(H))
     return dH, dW, db
 
 
-def _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate):
+def _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH):
     assert not accumulate or (("dW" not in need or dW is not None) and ("db" not in need or bias is None or db is not None)), \
         "accumulate needs the tensors to add to"
+    assert not accumulate_dH or "dH" not in need or dH is not None, "accumulate_dH needs the tensor to add to"
     dH = _grad_out(dH, "dH" in need, R, d, torch.bfloat16, H.device)
     dW = _grad_out(dW, "dW" in need, V, d, torch.bfloat16, H.device)
     if bias is None or "db" not in need:
@@ -366,15 +367,16 @@ def linear_distill_bwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teac
                        *, bias: Optional[torch.Tensor] = None, temperature: float = 1.0,
                        dloss: Optional[torch.Tensor] = None, scale: float = 1.0, dH: Optional[torch.Tensor] = None,
                        dW: Optional[torch.Tensor] = None, db: Optional[torch.Tensor] = None,
-                       need=("dH", "dW", "db"), accumulate: bool = False, workspace: Optional[torch.Tensor] = None):
+                       need=("dH", "dW", "db"), accumulate: bool = False, accumulate_dH: bool = False, workspace: Optional[torch.Tensor] = None):
     """Gradients of sum_r scale * dloss[r] * loss[r]; arguments and results as linear_nll_bwd."""
     R, V, d, ldh, ldw = _head_check(H, W, bias, idx, (teacher, lse, dloss))
     assert idx.dim() == 2 and teacher.shape == idx.shape
-    dH, dW, db = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate)
+    dH, dW, db = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH)
     ws, wsb = _ws(workspace)
     L.call("dgx_linear_distill_bwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), idx.data_ptr(),
            teacher.data_ptr(), idx.shape[1], float(temperature), lse.data_ptr(), _ptr(dloss), float(scale), R, V, d,
-           *_grad_args(dH), *_grad_args(dW), _ptr(db), int(accumulate), ws, wsb, _stream(H))
+           *_grad_args(dH), *_grad_args(dW), _ptr(db), int(accumulate) + 2 * int(accumulate_dH), ws, wsb,
+           _stream(H))
     return dH, dW, db
 
 

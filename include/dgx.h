@@ -404,8 +404,9 @@ dgx_status dgx_heads_to_rows(const void* src, void* dst, int ld, int col0, int B
  * each of them skipped when NULL; dH and dW DGX_F32 or DGX_BF16 with 16-byte
  * aligned rows. softmax - target is rounded to bf16 as the operand of the two
  * products (scale is applied after them, in fp32); db is summed unrounded.
- * accumulate = 1 adds to dW (fp32) and db. Every result is the same bits on
- * every run. workspace: dgx_linear_*_workspace_size() bytes, 128-byte aligned,
+ * accumulate: DGX_ACC_W adds to dW (fp32) and db, DGX_ACC_H to dH (fp32), so
+ * that several losses, heads or micro-batches sum into one gradient. Every
+ * result is the same bits on every run. workspace: dgx_linear_*_workspace_size() bytes, 128-byte aligned,
  * or NULL for the library's own buffer; its contents need not survive between
  * calls. Rows of H must be finite even where the row has no target (0 * inf in
  * dW); a row without a target has loss 0 and dH 0.
@@ -415,6 +416,7 @@ dgx_status dgx_heads_to_rows(const void* src, void* dst, int ld, int col0, int B
  * Joins dream_linear, log_softmax and nll_loss (runtime/ops/elementwise.inc:
  * 1432-1603) and their backward (runtime/ops/autograd.inc:156-245).
  */
+enum { DGX_ACC_W = 1, DGX_ACC_H = 2 };
 dgx_status dgx_linear_nll_fwd(const void* H, int ldh, const void* W, int ldw, const float* bias, const int* target,
                               int R, int V, int d, float* loss, float* lse, float* mean, void* workspace,
                               size_t workspace_bytes, void* stream);

@@ -41,7 +41,8 @@ def test_head_backward_refusals(lib):
     for kw in (dict(R=-1), dict(lse=None), dict(target=None), dict(dht=2), dict(dwt=3), dict(lddh=56),
                dict(lddh=66), dict(lddw=62), dict(dH=C.c_void_p(8)), dict(dW=C.c_void_p(8)), dict(ws=C.c_void_p(8))):
         assert nll_bwd(lib, **kw) == L.DGX_EINVAL, kw
-    assert nll_bwd(lib, acc=1) == L.DGX_EUNSUPPORTED
+    assert nll_bwd(lib, acc=1) == L.DGX_EUNSUPPORTED and nll_bwd(lib, acc=2) == L.DGX_EUNSUPPORTED
+    assert nll_bwd(lib, acc=4) == L.DGX_EINVAL
     assert nll_bwd(lib, wsb=8) == L.DGX_ENOMEM
     assert nll_bwd(lib, dH=None, dW=None) == L.DGX_OK  # nothing asked for
 

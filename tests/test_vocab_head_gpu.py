@@ -222,6 +222,22 @@ def test_fp32_gradients_accumulate_and_skip(dgx, K):
     assert dH._base[:, 96:].isnan().all()
 
 
+@pytest.mark.parametrize("R,V,d", [(300, 777, 96), (40, 20000, 64), (9000, 33000, 32)])
+def test_losses_sum_into_one_gradient(dgx, R, V, d):
+    """Hard and soft target on the same rows, the second call adding to the
+    first one's dH, dW and db (direct, sliced and pieced sums)."""
+    p = Problem(R, V, d, bias="plain", seed=21, scale=0.25 / R)
+    q = Problem(R, V, d, K=5, T=2.0, bias="plain", seed=21, scale=0.75 / R)
+    assert torch.equal(p.H, q.H) and torch.equal(p.W, q.W) and torch.equal(p.bias, q.bias)
+    out = dict(dH=torch.empty(R, d, device="cuda"), dW=torch.empty(V, d, device="cuda"),
+               db=torch.empty(V, device="cuda"))
+    p.bwd(dgx, p.fwd(dgx)[1], **out)
+    q.bwd(dgx, q.fwd(dgx)[1], accumulate=True, accumulate_dH=True, **out)
+    for name, a, b, ta, tb in (("dH", p.dH, q.dH, p.tol_dH, q.tol_dH), ("dW", p.dW, q.dW, p.tol_dW, q.tol_dW),
+                               ("db", p.db, q.db, p.tol_db, q.tol_db)):
+        within(out[name], a + b, ta + tb + U * 4 * (a.abs() + b.abs()), name)
+
+
 def test_all_rows_without_target(dgx):
     p = Problem(200, 500, 64, bias="plain", seed=2)
     p.target.fill_(-1)

@@ -212,45 +212,57 @@ __global__ void head_mean_kernel(const float* __restrict__ loss, int R, float* _
 // ---------------------------------------------------------------- backward
 constexpr int kSlabRows = 32;  // rows per partial column sum
 
-// db[j] (+)= scale * sum over slabs of dbp[slab][j]: a block owns 32 columns, its
-// 8 warps take the slabs in turn and are joined in warp order.
-__global__ void __launch_bounds__(256) head_db_kernel(const float* __restrict__ dbp, int slabs, int n, float scale,
-                                                      int accumulate, float* __restrict__ db) {
-  __shared__ float red[8][32];
-  dependents_may_start();
-  wait_for_predecessor();
+// What is left after the gradient products of a piece, in one launch: the first
+// blocks sum db, the others the slices of a product.
+struct SliceSum {  // out[r][j] (+)= scale * sum over slices of acc[slice][r][j], in order
+  const float* acc;
+  void* out;
+  int slices, rows, d, lda, bf16_out, add, ldo;  // pitches are multiples of four elements
+};
+struct BiasSum {  // db[j] (+)= scale * sum over slabs of dbp[slab][j]
+  const float* dbp;
+  float* db;
+  int slabs, n, add, blocks;
+};
+
+// A block owns 32 columns; its 8 warps take the slabs in turn and are joined in
+// warp order.
+__device__ __forceinline__ void bias_sum(const BiasSum& b, float scale, float (*red)[32]) {
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int j = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (j < n) {
+  if (j < b.n) {
 #pragma unroll 8
-    for (int i = w; i < slabs; i += 8) s += dbp[(size_t)i * n + j];
+    for (int i = w; i < b.slabs; i += 8) s += b.dbp[(size_t)i * b.n + j];
   }
   red[w][lane] = s;
   __syncthreads();
-  if (w == 0 && j < n) {
+  if (w == 0 && j < b.n) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) s += red[i][lane];
-    db[j] = (accumulate ? db[j] : 0.f) + scale * s;
+    b.db[j] = (b.add ? b.db[j] : 0.f) + scale * s;
   }
 }
 
-// out[r][j] (+)= scale * sum over slices of acc[slice][r][j], in order, rounded
-// once to bf16 where asked; four columns per thread (pitches are multiples of
-// four elements).
-__global__ void head_out_kernel(const float* __restrict__ acc, int slices, int rows, int d, int lda, float scale,
-                                int bf16_out, int accumulate, void* __restrict__ out, int ldo) {
+// Rounded once to bf16 where asked; four columns per thread.
+__global__ void __launch_bounds__(256) head_sums_kernel(SliceSum a, BiasSum b, float scale) {
+  __shared__ float red[8][32];
   wait_for_predecessor();
-  const int dq = (d + 3) >> 2;
-  const long long total = (long long)rows * dq;
-  const size_t slice = (size_t)rows * lda;
-  for (long long e = blockIdx.x * (long long)blockDim.x + threadIdx.x; e < total;
-       e += (long long)gridDim.x * blockDim.x) {
+  if (blockIdx.x < b.blocks) {
+    bias_sum(b, scale, red);
+    return;
+  }
+  const int dq = (a.d + 3) >> 2;
+  const long long total = (long long)a.rows * dq;
+  const size_t slice = (size_t)a.rows * a.lda;
+  for (long long e = (blockIdx.x - b.blocks) * (long long)blockDim.x + threadIdx.x; e < total;
+       e += (long long)(gridDim.x - b.blocks) * blockDim.x) {
     const long long r = e / dq;
     const int j = (int)(e - r * dq) * 4;
-    const float* p = acc + (size_t)r * lda + j;
+    const float* p = a.acc + (size_t)r * a.lda + j;
     float4 v = *reinterpret_cast<const float4*>(p);
-    for (int i = 1; i < slices; ++i) {
+#pragma unroll 4
+    for (int i = 1; i < a.slices; ++i) {
       const float4 u = *reinterpret_cast<const float4*>(p + i * slice);
       v.x += u.x;
       v.y += u.y;
@@ -258,15 +270,15 @@ __global__ void head_out_kernel(const float* __restrict__ acc, int slices, int r
       v.w += u.w;
     }
     const float f[4] = {scale * v.x, scale * v.y, scale * v.z, scale * v.w};
-    if (bf16_out) {
-      __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(out) + r * ldo + j;
-      if (j + 4 <= d)
+    if (a.bf16_out) {
+      __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.out) + r * a.ldo + j;
+      if (j + 4 <= a.d)
         *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
       else
-        for (int i = 0; j + i < d; ++i) o[i] = __float2bfloat16_rn(f[i]);
+        for (int i = 0; j + i < a.d; ++i) o[i] = __float2bfloat16_rn(f[i]);
     } else {
-      float* o = reinterpret_cast<float*>(out) + r * ldo + j;
-      for (int i = 0; i < 4 && j + i < d; ++i) o[i] = accumulate ? o[i] + f[i] : f[i];
+      float* o = reinterpret_cast<float*>(a.out) + r * a.ldo + j;
+      for (int i = 0; i < 4 && j + i < a.d; ++i) o[i] = a.add ? o[i] + f[i] : f[i];
     }
   }
 }
@@ -387,12 +399,10 @@ dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s) {
   return cuda_status(e, "head forward");
 }
 
-static cudaError_t launch_out(const float* acc, int slices, int rows, const HeadArgs& a, int lda, int bf16_out,
-                              int accumulate, void* out, int ldo, cudaStream_t s) {
-  const long long quads = (long long)rows * ((a.d + 3) / 4);
-  const unsigned blocks = (unsigned)std::min<long long>((quads + 255) / 256, num_sms() * 8ll);
-  return launch_dependent(head_out_kernel, blocks, 256, 0, 1, s, acc, slices, rows, a.d, lda, a.scale, bf16_out,
-                          accumulate, out, ldo);
+static cudaError_t launch_sums(const SliceSum& a, const BiasSum& b, float scale, cudaStream_t s) {
+  const long long quads = a.acc ? (long long)a.rows * ((a.d + 3) / 4) : 0;
+  const unsigned blocks = (unsigned)std::min<long long>((quads + 255) / 256, num_sms() * 8ll) + b.blocks;
+  return blocks ? launch_dependent(head_sums_kernel, blocks, 256, 0, 1, s, a, b, scale) : cudaSuccess;
 }
 
 dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
@@ -414,11 +424,6 @@ dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
     t.n = n;
     e = head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, true, g, p.pc, s);
     if (e != cudaSuccess) return cuda_status(e, "head backward");
-    if (a.db) {
-      e = launch_dependent(head_db_kernel, (n + 31) / 32, 256, 0, 1, s, dbp, p.slabs, n, a.scale, a.add_w,
-                           a.db + c0);
-      if (e != cudaSuccess) return cuda_status(e, "head backward");
-    }
     HeadGradTc m{};
     m.G = g;
     m.ldg = p.pc;
@@ -434,10 +439,17 @@ dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
     if (a.dH) m.out[0] = dh ? GradOut{dh, 0, c0 > 0, p.dp, p.sp.dh, 1.f} : GradOut{a.dH, a.dh_bf16, a.add_h, a.lddh, 1, a.scale};
     if (a.dW) m.out[1] = dw ? GradOut{dw, 0, 0, p.dp, p.sp.dw, 1.f} : GradOut{dw_out, a.dw_bf16, a.add_w, a.lddw, 1, a.scale};
     e = head_grads_tc(m, s);
-    if (e == cudaSuccess && a.dW && dw) e = launch_out(dw, p.sp.dw, n, a, p.dp, a.dw_bf16, a.add_w, dw_out, a.lddw, s);
+    if (e == cudaSuccess) {
+      SliceSum w{};
+      BiasSum b{};
+      if (a.dW && dw) w = SliceSum{dw, dw_out, p.sp.dw, n, a.d, p.dp, a.dw_bf16, a.add_w, a.lddw};
+      if (a.db) b = BiasSum{dbp, a.db + c0, p.slabs, n, a.add_w, (n + 31) / 32};
+      e = launch_sums(w, b, a.scale, s);
+    }
     if (e != cudaSuccess) return cuda_status(e, "head backward");
   }
-  if (a.dH && dh) e = launch_out(dh, p.sp.dh, a.R, a, p.dp, a.dh_bf16, a.add_h, a.dH, a.lddh, s);
+  if (a.dH && dh)
+    e = launch_sums(SliceSum{dh, a.dH, p.sp.dh, a.R, a.d, p.dp, a.dh_bf16, a.add_h, a.lddh}, BiasSum{}, a.scale, s);
   return cuda_status(e, "head backward");
 }
 

@@ -27,7 +27,8 @@ namespace {
 constexpr int HG_BM = 128;  // rows per CTA (256 per pair)
 constexpr int HG_BK = 64;
 constexpr int HG_STAGES = 6;
-constexpr int HG_THREADS = 192;
+constexpr int HG_EPI_WARPS = 8;
+constexpr int HG_THREADS = 64 + 32 * HG_EPI_WARPS;
 constexpr uint32_t HG_TMEM_COLS = 512;
 
 template <int BN>
@@ -35,11 +36,11 @@ struct HgCfg {
   static constexpr int A_BYTES = HG_BM * HG_BK * 2;
   static constexpr int B_BYTES = (BN / 2) * HG_BK * 2;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int SMEM = HG_STAGES * STAGE + 4 * 2 * 4096 + 1024 + 256;
+  static constexpr int SMEM = HG_STAGES * STAGE + HG_EPI_WARPS * 4096 + 1024 + 256;
 };
 
 struct GradProblem {
-  int tiles_m, nk, splits, kper, units;
+  int rows, tiles_m, nk, splits, kper, units;
   int out;      // 0 bf16 store, 1 fp32 store, 2 fp32 reduce-add
   float alpha;
 };
@@ -93,7 +94,7 @@ __global__ void __launch_bounds__(HG_THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* out_stage = smem + HG_STAGES * Cfg::STAGE;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_stage + 4 * 2 * 4096);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_stage + HG_EPI_WARPS * 4096);
   uint64_t* empty_bar = full_bar + HG_STAGES;
   uint64_t* accf_bar = empty_bar + HG_STAGES;  // [2]
   uint64_t* acce_bar = accf_bar + 2;           // [2]
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(HG_THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&accf_bar[b], 1);
-      mbar_init(&acce_bar[b], 8);
+      mbar_init(&acce_bar[b], 2 * HG_EPI_WARPS);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -202,9 +203,11 @@ __global__ void __launch_bounds__(HG_THREADS, 1)
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
-    const int q = warp & 3;
-    uint8_t* my_stage = out_stage + (warp - 2) * 2 * 4096;
+    // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
+    // Two warps per TMEM lane quarter take the column chunks in turn: a tile of
+    // few K steps lasts as long as its epilogue.
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* st = out_stage + (warp - 2) * 4096;
     uint32_t issued = 0, use = 0;
     Unit u;
     for (int i = 0; unit_at(a, i, pair, npairs, u); ++i) {
@@ -218,12 +221,12 @@ __global__ void __launch_bounds__(HG_THREADS, 1)
       const CUtensorMap* mo = u.prob ? &tmO1 : &tmO0;
       const int cw = g.out == 0 ? 64 : 32;
 #pragma unroll 1
-      for (int c = 0; c < BN; c += cw) {
+      for (int c = half * cw; c < BN; c += 2 * cw) {
         uint32_t r[64];
         tmem_ld32(taddr + c, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
         if (cw == 64) tmem_ld32(taddr + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
         tmem_ld_wait();
-        if (c + cw >= BN) {
+        if (c + 2 * cw >= BN) {  // this warp's last read of the accumulator
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -233,9 +236,8 @@ __global__ void __launch_bounds__(HG_THREADS, 1)
               mbar_arrive_remote(&acce_bar[buf], 0);
           }
         }
-        if (u.tn * BN + c >= a.d) continue;  // uniform: past the last column
-        uint8_t* st = my_stage + (issued & 1) * 4096;
-        if (lane == 0 && issued >= 2) bulk_wait_read1();
+        if (u.tn * BN + c >= a.d || row0 >= g.rows) continue;  // uniform: past the last column or row
+        if (lane == 0 && issued) bulk_wait_read0();
         __syncwarp();
         uint32_t w[32];
         if (cw == 64) {
@@ -299,13 +301,20 @@ cudaError_t launch(const CUtensorMap (&m)[6], const GradArgs& a, int pairs, cuda
 
 }  // namespace
 
+// K steps that a tile costs at least: its epilogue and the latency of its first
+// loads (4 / 7 / 10 / 14 / 20: 60 x 32000 x 1024 training 89 / 81 / 83 / 87 / 96
+// us, 333 x 50257 x 512 distillation 139 / 136 / 132 / 135 / 140, 16384 x 65 x 384
+// training 44 / 41 / 41 / 43 / 44).
+constexpr int kMinCost = 10;
+
 // Slices of the two products' sums so that no tile takes longer than the mean
 // load of an SM pair (at most kMaxSplits; the scratch is sized by the same rule).
 GradSplits head_grad_splits(int R, int n, int d, bool want_dh, bool want_dw) {
   const long long tn = (d + 255) / 256, pairs = std::max(1, num_sms() / 2);
   const long long kp[2] = {(n + 63) / 64, (R + 63) / 64};
   const long long tiles[2] = {want_dh ? (R + 255) / 256 * tn : 0, want_dw ? (n + 255) / 256 * tn : 0};
-  const long long mean = std::max<long long>(8, (tiles[0] * kp[0] + tiles[1] * kp[1] + pairs - 1) / pairs);
+  const long long work = tiles[0] * std::max<long long>(kp[0], kMinCost) + tiles[1] * std::max<long long>(kp[1], kMinCost);
+  const long long mean = std::max<long long>(8, (work + pairs - 1) / pairs);
   GradSplits sp;
   int* out[2] = {&sp.dh, &sp.dw};
   for (int i = 0; i < 2; ++i) {
@@ -337,6 +346,7 @@ cudaError_t head_grads_tc(const HeadGradTc& g, cudaStream_t s) {
     p.splits = std::max(1, o.splits);
     p.kper = (p.nk + p.splits - 1) / p.splits;
     if (!o.ptr) continue;
+    p.rows = rows[i];
     p.tiles_m = (rows[i] + 2 * HG_BM - 1) / (2 * HG_BM);
     p.units = p.tiles_m * a.tiles_n * p.splits;
     p.out = o.bf16 ? 0 : o.add ? 2 : 1;
@@ -351,7 +361,7 @@ cudaError_t head_grads_tc(const HeadGradTc& g, cudaStream_t s) {
   a.nl = a.p[1 - a.heavy].units;
   a.r = a.nh % P;
   if (a.r && a.nl) {
-    const int ch = a.p[a.heavy].kper, cl = a.p[1 - a.heavy].kper;
+    const int ch = std::max(a.p[a.heavy].kper, kMinCost), cl = std::max(a.p[1 - a.heavy].kper, kMinCost);
     a.x = std::min((ch + cl / 2) / cl, a.nl / (P - a.r));
   }
   return launch<BN>(m, a, P, s);

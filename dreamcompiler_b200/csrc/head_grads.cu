@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(HG_THREADS, 1)
             if (leader)
               mbar_arrive(&acce_bar[buf]);
             else
-              mbar_arrive_remote(&acce_bar[buf], 0);
+              mbar_arrive_remote_relaxed(&acce_bar[buf], 0);
           }
         }
         if (u.tn * BN + c >= a.d || row0 >= g.rows) continue;  // uniform: past the last column or row

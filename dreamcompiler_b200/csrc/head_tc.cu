@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
             if (leader)
               mbar_arrive(&acce_bar[buf]);
             else
-              mbar_arrive_remote(&acce_bar[buf], 0);
+              mbar_arrive_remote_relaxed(&acce_bar[buf], 0);
           }
         }
         const int n0 = nbase + c;   // column within the piece

@@ -65,4 +65,17 @@ __device__ __forceinline__ void mbar_arrive_remote(uint64_t* bar, uint32_t cta) 
       : "memory");
 }
 
+// The same without release semantics, for handing over a TMEM accumulator: its
+// reads are complete (tcgen05.wait::ld) and fenced (before_thread_sync), and no
+// memory write has to become visible with the arrival. A release at cluster
+// scope costs the arriving warp about 1600 cycles.
+__device__ __forceinline__ void mbar_arrive_remote_relaxed(uint64_t* bar, uint32_t cta) {
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\t"
+      "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
+      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(cta)
+      : "memory");
+}
+
 }  // namespace dgx

@@ -51,7 +51,7 @@ __device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepco
 // last (id kNoId, q 0). A teacher logit of -inf has q = 0; a row whose entries
 // are all absent or -inf has live = 0. The rank of an entry is the number of
 // entries before it, counted four ids per shared-memory load. start[row][s] is
-// the first entry whose id is at least 128 s. KI: entries per lane.
+// the first entry whose id is at least kHeadSlot s. KI: entries per lane.
 template <int KI>
 __global__ void __launch_bounds__(128) head_lists_kernel(const int* __restrict__ idx, const float* __restrict__ teacher,
                                                          int R, int V, int K, float inv_t, int* __restrict__ sid,
@@ -117,10 +117,10 @@ __global__ void __launch_bounds__(128) head_lists_kernel(const int* __restrict__
   if (lane == 0) live[row] = any ? 1.f : 0.f;
   __syncwarp();
   for (int t = lane; t < slots; t += 32) {
-    int lo = 0;  // entries below 128 t: a binary descent over KI * 32 entries
+    int lo = 0;  // entries below kHeadSlot t: a binary descent over KI * 32 entries
 #pragma unroll
     for (int step = KI * 32; step; step >>= 1)
-      if (lo + step <= KI * 32 && sorted[lo + step - 1] < t * 128) lo += step;
+      if (lo + step <= KI * 32 && sorted[lo + step - 1] < t * kHeadSlot) lo += step;
     start[(size_t)row * slots + t] = (uint16_t)min(lo, K);
   }
 }
@@ -295,7 +295,7 @@ int piece_cols(int R, int V) {
   return (int)std::min<long long>(std::max<long long>(c, 256), ((long long)V + 255) / 256 * 256);
 }
 
-int num_slots(int V) { return (int)(((long long)V + 255) / 256 * 2); }
+int num_slots(int V) { return (int)(((long long)V + 255) / 256 * (256 / kHeadSlot)); }
 
 struct Carve {
   char* p;
@@ -348,7 +348,7 @@ HeadTcArgs tc_args(const HeadArgs& a) {
 }  // namespace
 
 size_t head_fwd_scratch_bytes(int R, int V, int d, int K, bool lists) {
-  const int slots = std::max((V + 127) / 128, lists ? 0 : head_small_slots(R, V, d));
+  const int slots = std::max((V + 63) / 64, lists ? 0 : head_small_slots(R, V, d));
   return align128((size_t)slots * R * 8) + align128((size_t)R * K * 4) + (lists ? list_bytes(R, V, K) : 0);
 }
 
@@ -381,7 +381,8 @@ dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s) {
   Carve c{(char*)ws};
   HeadTcArgs t = tc_args(a);
   const int small = a.teacher ? 0 : head_small_slots(a.R, a.V, a.d);
-  const int slots = small ? small : (a.V + 127) / 128;
+  const int cols = head_stat_cols(a.d, a.bias != nullptr);
+  const int slots = small ? small : (a.V + cols - 1) / cols;
   t.part = c.take<float2>((size_t)slots * a.R);
   t.zs = c.take<float>((size_t)a.R * a.K);
   t.n = a.V;

@@ -10,6 +10,7 @@
 namespace dgx {
 
 constexpr int kHeadMaxK = 256;          // teacher entries per row
+constexpr int kHeadSlot = 64;          // columns per entry of a target list's start table
 constexpr int kHeadMaxRows = 1 << 23;   // rows, and columns of the vocabulary: tile counts fit 32 bits
 
 // One problem: logits z = (H . W^T + bias) / T of R rows over V columns, and a
@@ -47,16 +48,17 @@ struct HeadTcArgs {
   const float* bias;        // [V] or null
   const int* sid;           // [R][K] target ids, ascending when K > 1
   const float* sq;          // [R][K] their probabilities, or null (1)
-  const uint16_t* start;    // [R][slots] first entry with id >= 128 * slot, or null (K = 1)
+  const uint16_t* start;    // [R][slots] first entry with id >= kHeadSlot * slot, or null (K = 1)
   int slots;
   float* zs;                // [R][K] out: raw logits at the ids (statistics)
-  float2* part;             // [ceil(n / 128)][R] out: (max, sum) per 128 columns (statistics)
+  float2* part;             // [ceil(n / head_stat_cols())][R] out: (max, sum) per slot of columns (statistics)
   const float* live;        // [R] 0 where the row has no target, or null (id in [0, V))
   const float* dloss;       // [R] or null
   const float* lse;         // [R]
   float* dbp;               // [ceil(R / 32)][n] out: column sums per 32 rows, or null (gradient)
   uint32_t* err;
 };
+int head_stat_cols(int d, bool bias);  // columns per statistics slot: 64 or 128
 cudaError_t head_logits_tc(HeadTcArgs a, const void* H, int ldh, const void* W, int ldw, bool grad, void* g, int ldg,
                            cudaStream_t s);
 

@@ -3,14 +3,14 @@
 // tile over a CTA pair (cta_group::2, each SM its own 128 rows), consumed by
 // the epilogue where they stand. No logit is written to memory.
 //
-//   head_logits_kernel<kStats>   per row and 128 columns: max and sum of
+//   head_logits_kernel<kStats>   per row and warp: max and sum of
 //                                exp((z - max) / T), and z at the target's ids
 //   head_logits_kernel<kGrad>    G = w (exp(z/T - lse) - q) as bf16, and its
 //                                column sums before the rounding
 //
 // Both run the main loop of gemm2_kernel (TMA operand ring, one MMA-issuing
-// thread in the leader, two TMEM accumulators) with eight epilogue warps, two
-// per TMEM lane quarter, each taking 128 of the tile's 256 columns.
+// thread in the leader, two TMEM accumulators) with eight or sixteen epilogue
+// warps.
 #include <algorithm>
 
 #include "gemm.h"
@@ -26,20 +26,36 @@ constexpr int HD_BM = 128;  // rows per CTA (256 per pair)
 constexpr int HD_BN = 256;  // vocabulary columns per tile (128 W rows loaded per CTA)
 constexpr int HD_BK = 64;   // one 128-byte swizzled row of bf16
 constexpr int HD_STAGE = 2 * HD_BM * HD_BK * 2;  // 16 KB of H and 16 KB of W
-constexpr int HD_EPI_WARPS = 8;
-constexpr int HD_THREADS = 64 + 32 * HD_EPI_WARPS;
 constexpr uint32_t HD_TMEM_COLS = 512;
 
 constexpr int kStats = 0, kGrad = 1;
-// Per epilogue warp, after the operand stages: a 4 KB staging box for G (the
-// gradient), and the bias of its 128 columns. Both and six stages do not fit.
-template <int MODE, bool BIAS>
+// EW epilogue warps; a TMEM lane quarter's 256 columns are split over the
+// quarter's warps. After the operand stages: a 4 KB staging box for G per
+// warp (the gradient), and each warp's columns of the bias.
+template <int MODE, bool BIAS, int EW>
 struct HdCfg {
-  static constexpr int STAGES = MODE == kGrad && BIAS ? 5 : 6;
-  static constexpr int OUT = MODE == kGrad ? HD_EPI_WARPS * 4096 : 0;
-  static constexpr int BIAS_BYTES = BIAS ? HD_EPI_WARPS * 512 : 0;
-  static constexpr int SMEM = STAGES * HD_STAGE + OUT + BIAS_BYTES + 1024 + 256;
+  static constexpr int COLS = 4 * HD_BN / EW;
+  static constexpr int THREADS = 64 + 32 * EW;
+  static constexpr int OUT = MODE == kGrad ? EW * 4096 : 0;
+  static constexpr int BIAS_BYTES = BIAS ? 4 * HD_BN * 4 : 0;
+  static constexpr int TAIL = OUT + BIAS_BYTES + 1024 + 256;
+  static constexpr int FIT = (232448 - TAIL) / HD_STAGE;
+  static constexpr int STAGES = FIT < 6 ? FIT : 6;
+  static constexpr int SMEM = STAGES * HD_STAGE + TAIL;
 };
+// How many: the exponentials, sums and moves of a 256 x 256 tile take eight
+// warps about 4100 cycles (statistics) to 7000 (gradient with bias sums), mostly
+// waiting for one another's results; sixteen, with half the registers each,
+// need about two thirds of that. A tile's MMAs take 8 d cycles, so sixteen are
+// faster up to d = 640, or 768 with a bias (whole training pass, 8 against 16
+// warps: 333 x 50257 x 512 129 / 121 us, 8192 x 4000 x 256 101 / 96,
+// 2000 x 20000 x 640 with bias 189 / 183, 1537 x 50257 x 768 with bias 405 /
+// 400), and beyond that eight, whose smaller staging leaves an operand stage
+// more (1000 x 32000 x 768 157 / 160, 2000 x 20000 x 896 with bias 236 / 237,
+// 4096 x 32768 x 1024 742 / 753).
+constexpr int kManyWarps = 16, kFewWarps = 8;
+bool many_warps(int d, bool bias) { return d <= (bias ? 768 : 640); }
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -151,13 +167,14 @@ __device__ __forceinline__ void column_sums(float (&z)[32], int lane) {
   }
 }
 
-template <int MODE, bool BIAS>
-__global__ void __launch_bounds__(HD_THREADS, 1)
+template <int MODE, bool BIAS, int HD_EPI_WARPS>
+__global__ void __launch_bounds__(64 + 32 * HD_EPI_WARPS, 1)
     head_logits_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW,
                        const __grid_constant__ CUtensorMap tmG, HeadTcArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  using Cfg = HdCfg<MODE, BIAS>;
+  using Cfg = HdCfg<MODE, BIAS, HD_EPI_WARPS>;
+  constexpr int COLS = Cfg::COLS;
   constexpr int HD_STAGES = Cfg::STAGES;
   uint8_t* out_stage = smem + HD_STAGES * HD_STAGE;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_stage + Cfg::OUT + Cfg::BIAS_BYTES);
@@ -268,18 +285,18 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
+    // ------------------------------------------------------------ epilogue (the other warps, both CTAs)
     const int q = warp & 3;              // TMEM lane quarter this warp may access
-    const int half = (warp - 2) >> 2;    // its 128 columns of the tile
+    const int part = (warp - 2) >> 2;    // its columns of the tile
     uint8_t* st = out_stage + (warp - 2) * 4096;
-    float* bias_s = reinterpret_cast<float*>(out_stage + Cfg::OUT) + (warp - 2) * 128;
+    float* bias_s = reinterpret_cast<float*>(out_stage + Cfg::OUT) + (warp - 2) * COLS;
     uint32_t issued = 0, use = 0;
     for (int t = pair; t < num_tiles; t += npairs, ++use) {
       const int buf = use & 1;
       int tm, tn;
       coords(t, tm, tn);
       const int row0 = tm * 2 * HD_BM + (int)rank * HD_BM + q * 32, row = row0 + lane;
-      const int nbase = tn * HD_BN + half * 128;  // first column of this warp, within the piece
+      const int nbase = tn * HD_BN + part * COLS;  // first column of this warp, within the piece
       const bool row_ok = row < a.R;
       // the row's target entries from this warp's columns on
       Target tg{nullptr, nullptr, 0, 0, Target::kNone, Target::kNone, 0.f, 0.f};
@@ -288,7 +305,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
         tg.ids = a.sid + (size_t)row * a.K;
         tg.qs = a.sq ? a.sq + (size_t)row * a.K : nullptr;
         tg.K = a.K;
-        tg.start(a.start ? a.start[(size_t)row * a.slots + (a.c0 + nbase) / 128] : 0);
+        tg.start(a.start ? a.start[(size_t)row * a.slots + (a.c0 + nbase) / kHeadSlot] : 0);
         if (MODE == kGrad) {
           const bool live = a.live ? a.live[row] != 0.f : (tg.nid >= 0 && tg.nid < a.V);
           w = live ? (a.dloss ? a.dloss[row] : 1.f) : 0.f;
@@ -298,31 +315,25 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
         w = 0.f;
       }
       if constexpr (BIAS) {  // loaded while the accumulator is still being filled
-        float4 b;
-        const int j = nbase + lane * 4;
-        b.x = j < a.n ? __ldg(a.bias + a.c0 + j) : 0.f;
-        b.y = j + 1 < a.n ? __ldg(a.bias + a.c0 + j + 1) : 0.f;
-        b.z = j + 2 < a.n ? __ldg(a.bias + a.c0 + j + 2) : 0.f;
-        b.w = j + 3 < a.n ? __ldg(a.bias + a.c0 + j + 3) : 0.f;
-        *reinterpret_cast<float4*>(bias_s + lane * 4) = b;
+#pragma unroll
+        for (int j = lane; j < COLS; j += 32) bias_s[j] = nbase + j < a.n ? __ldg(a.bias + a.c0 + nbase + j) : 0.f;
         __syncwarp();
       }
       if (!mbar_wait(&accf_bar[buf], (use >> 1) & 1, wc)) break;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + buf * HD_BN + half * 128;
+      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + buf * HD_BN + part * COLS;
       float m = -INFINITY, s = 0.f;
-      // 32 columns at a time; the next 32 are on their way from TMEM meanwhile
-      uint32_t r[32];
-      tmem_ld32(taddr, r);
 #pragma unroll 1
-      for (int c = 0; c < 128; c += 32) {
-        tmem_ld_wait();
+      for (int c = 0; c < COLS; c += 32) {
         float z[32];
+        {
+          uint32_t r[32];
+          tmem_ld32(taddr + c, r);
+          tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(r[j]);
-        if (c < 96) {
-          tmem_ld32(taddr + c + 32, r);
-        } else {  // this warp's last read of the accumulator
+          for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(r[j]);
+        }
+        if (c + 32 == COLS) {  // this warp's last read of the accumulator
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -374,7 +385,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
           }
         }
       }
-      if (MODE == kStats && row_ok && nbase < a.n) a.part[(size_t)(tn * 2 + half) * a.R + row] = make_float2(m, s);
+      if (MODE == kStats && row_ok && nbase < a.n) a.part[(size_t)(nbase / COLS) * a.R + row] = make_float2(m, s);
     }
     if (MODE == kGrad && lane == 0) bulk_wait0();
   }
@@ -391,6 +402,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
 }
 
 }  // namespace
+
+int head_stat_cols(int d, bool bias) { return 4 * HD_BN / (many_warps(d, bias) ? kManyWarps : kFewWarps); }
 
 // Logits of the piece [c0, c0 + n) of the vocabulary: row statistics
 // (grad = false) or G (grad = true, into g with pitch ldg).
@@ -410,16 +423,20 @@ cudaError_t head_logits_tc(HeadTcArgs a, const void* H, int ldh, const void* W, 
   // 6.74 -> 6.58 ms, 4096 x 32768 x 1024 874 -> 863 us with one group).
   a.group_m = (int)std::max<long long>(8, (48ll << 20) / (2ll * HD_BM * 2 * a.d));
   const int pairs = (int)std::min<long long>((long long)a.tiles_m * a.tiles_n, num_sms() / 2);
-  auto run = [&](auto kern, int smem, std::atomic<unsigned long long>& done) {
-    const cudaError_t e = allow_smem(kern, smem, done);
-    return e != cudaSuccess ? e : launch_dependent(kern, 2 * pairs, HD_THREADS, smem, 2, s, mh, mw, mg, a);
+  auto run = [&](auto mode, auto bias, auto warps) {
+    constexpr int M = decltype(mode)::value, EW = decltype(warps)::value;
+    constexpr bool B = decltype(bias)::value != 0;
+    using Cfg = HdCfg<M, B, EW>;
+    static std::atomic<unsigned long long> done;
+    const cudaError_t e = allow_smem(head_logits_kernel<M, B, EW>, Cfg::SMEM, done);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(head_logits_kernel<M, B, EW>, 2 * pairs, Cfg::THREADS, Cfg::SMEM, 2, s, mh, mw, mg, a);
   };
-  static std::atomic<unsigned long long> done[4];
-  if (grad)
-    return a.bias ? run(head_logits_kernel<kGrad, true>, HdCfg<kGrad, true>::SMEM, done[0])
-                  : run(head_logits_kernel<kGrad, false>, HdCfg<kGrad, false>::SMEM, done[1]);
-  return a.bias ? run(head_logits_kernel<kStats, true>, HdCfg<kStats, true>::SMEM, done[2])
-                : run(head_logits_kernel<kStats, false>, HdCfg<kStats, false>::SMEM, done[3]);
+  auto with_warps = [&](auto mode, auto bias) {
+    return many_warps(a.d, a.bias != nullptr) ? run(mode, bias, IntC<kManyWarps>{}) : run(mode, bias, IntC<kFewWarps>{});
+  };
+  if (grad) return a.bias ? with_warps(IntC<kGrad>{}, IntC<1>{}) : with_warps(IntC<kGrad>{}, IntC<0>{});
+  return a.bias ? with_warps(IntC<kStats>{}, IntC<1>{}) : with_warps(IntC<kStats>{}, IntC<0>{});
 }
 
 }  // namespace dgx

@@ -83,7 +83,8 @@ dgx_status run_bwd(const char* op, HeadArgs& a, int dh_type, int dw_type, int ac
 }
 
 dgx_status check_temperature(const char* op, float t) {
-  if (!(t > 0.f) || !std::isfinite(t) || !std::isfinite(1.f / t))
+  // T^2 and the scaled logits' factor log2(e) / T have to be finite too
+  if (!(t > 0.f) || !std::isfinite(t * t) || !std::isfinite(2.f / t))
     return set_error(DGX_EINVAL, "%s: temperature %g", op, (double)t);
   return DGX_OK;
 }

@@ -60,7 +60,7 @@ def test_distill_refusals(lib):
 
     for f in (fwd, bwd):
         for kw in (dict(K=0), dict(K=257), dict(T=0.0), dict(T=-2.0), dict(T=float("nan")), dict(T=float("inf")),
-                   dict(T=1e-45), dict(teacher=None)):
+                   dict(T=1e-45), dict(T=4e-39), dict(T=2e19), dict(teacher=None)):
             assert f(**kw) == L.DGX_EINVAL, kw
     assert fwd(idx=None) == L.DGX_EINVAL and bwd(lse=None) == L.DGX_EINVAL
 

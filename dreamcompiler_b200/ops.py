@@ -245,6 +245,9 @@ def linear_distill_workspace_size(R: int, V: int, d: int, K: int, backward: bool
     return L.load().dgx_linear_distill_workspace_size(R, V, d, K, int(backward))
 
 
+_ROW_DT = {torch.float32: L.DGX_F32, torch.bfloat16: L.DGX_BF16}
+
+
 def _ws(workspace: Optional[torch.Tensor]):
     return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
 
@@ -269,20 +272,18 @@ def _head_check(H, W, bias, rows32, rowsf):
     return R, V, d, ldh if R > 1 else (d + 7) // 8 * 8, ldw if V > 1 else (d + 7) // 8 * 8
 
 
-def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
-
-
-def _grad_out(out, want: bool, rows: int, d: int, dtype, device):
-    """The tensor a gradient goes to: the caller's, a new one (rows padded to 16 bytes), or None."""
+def _grad_out(out, want: bool, rows: int, d: int, device, dev: int):
+    """A gradient's tensor (the caller's; a new bf16 one, its rows padded to 16
+    bytes; or None) and its pointer, type and pitch."""
     if not want:
-        return None
+        return None, None, L.DGX_BF16, 0
+    dp = (d + 7) // 8 * 8
     if out is None:
-        dp = (d + 7) // 8 * 8
-        out = torch.empty(rows, dp, device=device, dtype=dtype)
-        return out if dp == d else out[:, :d]
-    assert out.device == device and out.shape == (rows, d) and (out.stride(1) == 1 or d == 1) and out.dtype in _DT
-    return out
+        out = torch.empty(rows, dp, device=device, dtype=torch.bfloat16)
+        return out if dp == d else out[:, :d], out.data_ptr(), L.DGX_BF16, dp
+    code, (ld, sc) = _ROW_DT.get(out.dtype), out.stride()
+    assert code is not None and out.get_device() == dev and out.shape == (rows, d) and (sc == 1 or d == 1)
+    return out, out.data_ptr(), code, ld if rows > 1 else dp
 
 
 def linear_nll_fwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
@@ -315,31 +316,30 @@ def linear_nll_bwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, lse: 
     bias) are None. dH and dW are new bf16 tensors unless given (bf16 or fp32);
     accumulate adds to the given fp32 dW and db, accumulate_dH to the fp32 dH."""
     R, V, d, ldh, ldw = _head_check(H, W, bias, target, (lse, dloss))
-    dH, dW, db = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH)
+    dH, dW, db, grads = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH)
     ws, wsb = _ws(workspace)
     L.call("dgx_linear_nll_bwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), target.data_ptr(),
-           lse.data_ptr(), _ptr(dloss), float(scale), R, V, d, *_grad_args(dH), *_grad_args(dW), _ptr(db),
+           lse.data_ptr(), _ptr(dloss), float(scale), R, V, d, *grads,
            int(accumulate) + 2 * int(accumulate_dH), ws, wsb, _stream(H))
     return dH, dW, db
 
 
 def _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH):
-    assert not accumulate or (("dW" not in need or dW is not None) and ("db" not in need or bias is None or db is not None)), \
-        "accumulate needs the tensors to add to"
-    assert not accumulate_dH or "dH" not in need or dH is not None, "accumulate_dH needs the tensor to add to"
-    dH = _grad_out(dH, "dH" in need, R, d, torch.bfloat16, H.device)
-    dW = _grad_out(dW, "dW" in need, V, d, torch.bfloat16, H.device)
+    """The gradients' tensors (dH, dW, db) and their arguments in the C call's order."""
+    if accumulate or accumulate_dH:
+        assert not accumulate or (("dW" not in need or dW is not None) and ("db" not in need or bias is None or db is not None)), \
+            "accumulate needs the tensors to add to"
+        assert not accumulate_dH or "dH" not in need or dH is not None, "accumulate_dH needs the tensor to add to"
+    device, dev = H.device, H.get_device()
+    dH, hp, ht, hl = _grad_out(dH, "dH" in need, R, d, device, dev)
+    dW, wp, wt, wl = _grad_out(dW, "dW" in need, V, d, device, dev)
     if bias is None or "db" not in need:
-        db = None
-    elif db is None:
-        db = torch.empty(V, device=H.device, dtype=torch.float32)
+        return dH, dW, None, (hp, ht, hl, wp, wt, wl, None)
+    if db is None:
+        db = torch.empty(V, device=device, dtype=torch.float32)
     else:
-        assert db.device == H.device and db.dtype == torch.float32 and db.is_contiguous() and db.numel() == V
-    return dH, dW, db
-
-
-def _grad_args(t):
-    return (None, L.DGX_BF16, 0) if t is None else (t.data_ptr(), _DT[t.dtype], _pitch(t))
+        assert db.get_device() == dev and db.dtype is torch.float32 and db.is_contiguous() and db.numel() == V
+    return dH, dW, db, (hp, ht, hl, wp, wt, wl, db.data_ptr())
 
 
 def linear_distill_fwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,
@@ -371,16 +371,13 @@ def linear_distill_bwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teac
     """Gradients of sum_r scale * dloss[r] * loss[r]; arguments and results as linear_nll_bwd."""
     R, V, d, ldh, ldw = _head_check(H, W, bias, idx, (teacher, lse, dloss))
     assert idx.dim() == 2 and teacher.shape == idx.shape
-    dH, dW, db = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH)
+    dH, dW, db, grads = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH)
     ws, wsb = _ws(workspace)
     L.call("dgx_linear_distill_bwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), idx.data_ptr(),
            teacher.data_ptr(), idx.shape[1], float(temperature), lse.data_ptr(), _ptr(dloss), float(scale), R, V, d,
-           *_grad_args(dH), *_grad_args(dW), _ptr(db), int(accumulate) + 2 * int(accumulate_dH), ws, wsb,
+           *grads, int(accumulate) + 2 * int(accumulate_dH), ws, wsb,
            _stream(H))
     return dH, dW, db
-
-
-_ROW_DT = {torch.float32: L.DGX_F32, torch.bfloat16: L.DGX_BF16}
 
 
 def embed_fwd(tok: torch.Tensor, W: torch.Tensor, *, scale: float = 1.0, pos: Optional[torch.Tensor] = None,

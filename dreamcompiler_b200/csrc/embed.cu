@@ -571,6 +571,71 @@ __global__ void __launch_bounds__(256, 4) embed_sum_kernel(const TG* __restrict_
   }
 }
 
+// ---------------------------------------------------------------- few tokens
+// Up to kFew tokens need no sort: a block owns 32 table rows and 256 columns,
+// reads all ids, keeps those of its rows in order, and each warp sums and
+// writes (or zeroes) four rows. One launch instead of three; the rows of one
+// token are added by one warp, which bounds kFew (128 equal ids: 16 rounds of
+// loads).
+constexpr int kFew = 128;
+
+template <typename TG, typename TW, bool VEC>
+__global__ void __launch_bounds__(256) embed_few_kernel(const int* __restrict__ tok, const TG* __restrict__ dx,
+                                                        TW* __restrict__ dW, SumArgs a) {
+  __shared__ int pos_s[kFew], row_s[kFew], mine_s[8][kFew], count_s[4];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t0 = blockIdx.x * 32, c0 = blockIdx.y * kSlab, left = a.d - c0;
+  const unsigned lt = (1u << lane) - 1;
+  unsigned hits = 0;
+  int row = -1;
+  if (w < kFew / 32) {
+    const unsigned t = threadIdx.x < a.n ? (unsigned)tok[threadIdx.x] : 0xffffffffu;
+    if (t < (unsigned)a.V && t - (unsigned)t0 < 32u) row = (int)(t - t0);
+    hits = __ballot_sync(0xffffffffu, row >= 0);
+    if (lane == 0) count_s[w] = __popc(hits);
+  }
+  __syncthreads();
+  int total = 0, at = 0;
+#pragma unroll
+  for (int i = 0; i < kFew / 32; ++i) {
+    if (i < w) at += count_s[i];
+    total += count_s[i];
+  }
+  if (row >= 0) {
+    pos_s[at + __popc(hits & lt)] = threadIdx.x;
+    row_s[at + __popc(hits & lt)] = row;
+  }
+  __syncthreads();
+  for (int r = w; r < 32 && t0 + r < a.V; r += 8) {
+    int cnt = 0;
+    for (int c = 0; c < total; c += 32) {
+      const bool is = c + lane < total && row_s[c + lane] == r;
+      const unsigned m = __ballot_sync(0xffffffffu, is);
+      if (is) mine_s[w][cnt + __popc(m & lt)] = pos_s[c + lane];
+      cnt += __popc(m);
+    }
+    __syncwarp();
+    if (a.accumulate && !cnt) continue;
+    constexpr int kUnroll = 8;
+    float acc[8] = {};
+    for (int j = 0; j < cnt; j += kUnroll) {
+      Row8<TG, VEC> v[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (j + u < cnt) v[u].load(dx + (size_t)mine_s[w][j + u] * a.lddx + c0, lane, left);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (j + u < cnt) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k] += v[u].get(k);
+        }
+    }
+    finish_row<TW, VEC>(a, dW, t0 + r, c0, lane, acc);
+    __syncwarp();  // mine_s is reused
+  }
+}
+
 bool type_ok(int t) { return t == DGX_F32 || t == DGX_BF16; }
 int type_size(int t) { return t == DGX_F32 ? 4 : 2; }
 
@@ -586,10 +651,14 @@ struct Layout {
   size_t a, b, rank, counters, parts, bytes;
 };
 Layout layout(int n, int d) {
-  Layout l;
+  Layout l{};
   l.blocks = (int)(((long long)n + kBlockPos - 1) / kBlockPos);
   l.slabs = (d + kSlab - 1) / kSlab;
   size_t o = 0;
+  if (n <= kFew) {  // no sort, no parts
+    l.bytes = 0;
+    return l;
+  }
   l.a = o, o += align16((size_t)n * 8);
   l.b = o, o += align16((size_t)n * 8);
   l.rank = o, o += align16((size_t)n * 4);
@@ -646,7 +715,10 @@ cudaError_t launch_zero(const ZeroArgs& a, cudaStream_t s) {
 }
 
 template <typename TG, typename TW, bool VEC>
-cudaError_t launch_sum(const void* dx, void* dW, const SumArgs& a, int blocks, cudaStream_t s) {
+cudaError_t launch_sum(const int* tok, const void* dx, void* dW, const SumArgs& a, int blocks, cudaStream_t s) {
+  if (a.n <= kFew)
+    return launch_dependent(embed_few_kernel<TG, TW, VEC>, dim3((a.V + 31) / 32, a.slabs), 256, 0, 1, s, tok,
+                            (const TG*)dx, (TW*)dW, a);
   return launch_dependent(embed_sum_kernel<TG, TW, VEC>, blocks, 256, 0, 1, s, (const TG*)dx, (TW*)dW, a);
 }
 
@@ -711,60 +783,62 @@ dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int 
     return cuda_status(cudaMemset2DAsync(dW, lddw * es, 0, d * es, V, s), "dgx_embed_bwd");
   }
   const Layout l = layout(n, d);
-  if ((long long)l.blocks * l.slabs > 0x7fffffffll)
+  if ((long long)l.blocks * l.slabs > 0x7fffffffll || l.slabs > 65535)
     return set_error(DGX_EINVAL, "dgx_embed_bwd: n=%d V=%d d=%d too large", n, V, d);
   char* ws = (char*)workspace;
   if (ws && workspace_bytes < l.bytes)
     return set_error(DGX_ENOMEM, "dgx_embed_bwd: workspace %zu bytes < %zu", workspace_bytes, l.bytes);
   if (ws && ((uintptr_t)ws & 15)) return set_error(DGX_EINVAL, "dgx_embed_bwd: workspace must be 16-byte aligned");
-  if (!ws) ws = (char*)library_scratch(l.bytes, s);
-  if (!ws) return set_error(DGX_ENOMEM, "dgx_embed_bwd: cannot allocate %zu bytes of scratch", l.bytes);
-  SortArgs so{};
-  so.tok = tok;
-  so.n = n;
-  so.V = V;
-  int kb = 1;
-  while (kb < 31 && (V >> kb)) ++kb;  // keys 0 .. V
-  so.passes = (kb + kMaxDigitBits - 1) / kMaxDigitBits;
-  so.bits = (kb + so.passes - 1) / so.passes;
-  so.a = (int2*)(ws + l.a);
-  so.b = (int2*)(ws + l.b);
-  so.rank = (int*)(ws + l.rank);
-  so.counters = (int*)(ws + l.counters);
-  so.ncounters = l.blocks * l.slabs;
-  cudaError_t e = launch_sort(so, s);
-  if (e != cudaSuccess) return cuda_status(e, "dgx_embed_bwd");
-  if (!accumulate) {
-    ZeroArgs z{tok, n, V, (char*)dW, (size_t)lddw * type_size(dw_type), d * type_size(dw_type), 0};
-    z.vec = (((uintptr_t)dW | z.pitch | (size_t)z.row_bytes) & 15) == 0;
-    e = launch_zero(z, s);
-    if (e != cudaSuccess) return cuda_status(e, "dgx_embed_bwd");
-  }
   SumArgs a{};
-  a.sorted = so.passes & 1 ? so.a : so.b;
-  a.counters = so.counters;
-  a.parts = (float*)(ws + l.parts);
   a.n = n;
   a.d = d;
   a.V = V;
   a.slabs = l.slabs;
   a.blocks = l.blocks;
-  const int blocks = l.blocks * l.slabs;
   a.lddx = lddx;
   a.lddw = lddw;
   a.accumulate = accumulate ? 1 : 0;
   a.scale = scale;
+  cudaError_t e = cudaSuccess;
+  if (n > kFew) {
+    if (!ws) ws = (char*)library_scratch(l.bytes, s);
+    if (!ws) return set_error(DGX_ENOMEM, "dgx_embed_bwd: cannot allocate %zu bytes of scratch", l.bytes);
+    SortArgs so{};
+    so.tok = tok;
+    so.n = n;
+    so.V = V;
+    int kb = 1;
+    while (kb < 31 && (V >> kb)) ++kb;  // keys 0 .. V
+    so.passes = (kb + kMaxDigitBits - 1) / kMaxDigitBits;
+    so.bits = (kb + so.passes - 1) / so.passes;
+    so.a = (int2*)(ws + l.a);
+    so.b = (int2*)(ws + l.b);
+    so.rank = (int*)(ws + l.rank);
+    so.counters = (int*)(ws + l.counters);
+    so.ncounters = l.blocks * l.slabs;
+    e = launch_sort(so, s);
+    if (e == cudaSuccess && !accumulate) {
+      ZeroArgs z{tok, n, V, (char*)dW, (size_t)lddw * type_size(dw_type), d * type_size(dw_type), 0};
+      z.vec = (((uintptr_t)dW | z.pitch | (size_t)z.row_bytes) & 15) == 0;
+      e = launch_zero(z, s);
+    }
+    if (e != cudaSuccess) return cuda_status(e, "dgx_embed_bwd");
+    a.sorted = so.passes & 1 ? so.a : so.b;
+    a.counters = so.counters;
+    a.parts = (float*)(ws + l.parts);
+  }
+  const int blocks = l.blocks * l.slabs;
   const bool vec = vec_ok(dx, dx_type, lddx, d) && vec_ok(dW, dw_type, lddw, d);
   const bool g32 = dx_type == DGX_F32, w32 = dw_type == DGX_F32;
   if (g32 && w32)
-    e = vec ? launch_sum<float, float, true>(dx, dW, a, blocks, s) : launch_sum<float, float, false>(dx, dW, a, blocks, s);
+    e = vec ? launch_sum<float, float, true>(tok, dx, dW, a, blocks, s) : launch_sum<float, float, false>(tok, dx, dW, a, blocks, s);
   else if (g32)
-    e = vec ? launch_sum<float, __nv_bfloat16, true>(dx, dW, a, blocks, s) : launch_sum<float, __nv_bfloat16, false>(dx, dW, a, blocks, s);
+    e = vec ? launch_sum<float, __nv_bfloat16, true>(tok, dx, dW, a, blocks, s) : launch_sum<float, __nv_bfloat16, false>(tok, dx, dW, a, blocks, s);
   else if (w32)
-    e = vec ? launch_sum<__nv_bfloat16, float, true>(dx, dW, a, blocks, s) : launch_sum<__nv_bfloat16, float, false>(dx, dW, a, blocks, s);
+    e = vec ? launch_sum<__nv_bfloat16, float, true>(tok, dx, dW, a, blocks, s) : launch_sum<__nv_bfloat16, float, false>(tok, dx, dW, a, blocks, s);
   else
-    e = vec ? launch_sum<__nv_bfloat16, __nv_bfloat16, true>(dx, dW, a, blocks, s)
-            : launch_sum<__nv_bfloat16, __nv_bfloat16, false>(dx, dW, a, blocks, s);
+    e = vec ? launch_sum<__nv_bfloat16, __nv_bfloat16, true>(tok, dx, dW, a, blocks, s)
+            : launch_sum<__nv_bfloat16, __nv_bfloat16, false>(tok, dx, dW, a, blocks, s);
   return cuda_status(e, "dgx_embed_bwd");
 }
 

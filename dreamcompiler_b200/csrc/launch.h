@@ -13,10 +13,10 @@ namespace dgx {
 // before it ends), so the stream's order holds. cluster > 1: thread-block
 // clusters of that many CTAs.
 template <typename... P, typename... A>
-cudaError_t launch_dependent(void (*kern)(P...), unsigned blocks, int threads, int smem, int cluster, cudaStream_t s,
+cudaError_t launch_dependent(void (*kern)(P...), dim3 blocks, int threads, int smem, int cluster, cudaStream_t s,
                              const A&... args) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks);
+  cfg.gridDim = blocks;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;

@@ -10,6 +10,8 @@ two launches of each kernel).
     python -m dreamcompiler_b200.profile_case gpt                     # one config-3 training step
     python -m dreamcompiler_b200.profile_case linear                  # GPT MLP-up: 16384x1536x384 + bias
     python -m dreamcompiler_b200.profile_case gemm_f64 --n 4096       # f64 DFMA GEMM
+    python -m dreamcompiler_b200.profile_case head                    # head loss, 4096 rows x 32768 x 1024
+    python -m dreamcompiler_b200.profile_case embed                   # embedding, 16384 tokens, 50257 x 1024
 """
 from __future__ import annotations
 
@@ -21,7 +23,7 @@ def main() -> None:
     import dreamcompiler_b200 as dgx
 
     ap = argparse.ArgumentParser()
-    ap.add_argument("kind", choices=["flash", "gemm", "w8", "gemm_f32", "conv", "gpt", "linear", "gemm_f64"])
+    ap.add_argument("kind", choices=["flash", "gemm", "w8", "gemm_f32", "conv", "gpt", "linear", "gemm_f64", "head", "embed"])
     ap.add_argument("--bh", type=int, default=16)
     ap.add_argument("--seq", type=int, default=2048)
     ap.add_argument("--dim", type=int, default=64)
@@ -50,6 +52,24 @@ def main() -> None:
         Y = torch.empty(16384, 1536, device="cuda", dtype=torch.bfloat16)
         for _ in range(a.reps):
             dgx.gemm(X, W, transB=True, out=Y, bias=b)
+    elif a.kind == "head":
+        R, V, d = 4096, 32768, 1024
+        H = torch.randn(R, d, device="cuda", generator=g).bfloat16()
+        W = (torch.randn(V, d, device="cuda", generator=g) * 3 / d ** 0.5).bfloat16()
+        t = torch.randint(0, V, (R,), device="cuda", dtype=torch.int32, generator=g)
+        for _ in range(a.reps):
+            _, lse = dgx.linear_nll_fwd(H, W, t)
+            dgx.linear_nll_bwd(H, W, t, lse, scale=1 / R)
+    elif a.kind == "embed":  # ids with P(rank r) ~ 1 / r, bf16 activations, fp32 table
+        n, V, d = 16384, 50257, 1024
+        cdf = torch.cumsum(1.0 / torch.arange(1, V + 1, device="cuda", dtype=torch.float64), 0)
+        ranks = torch.searchsorted(cdf, torch.rand(n, device="cuda", dtype=torch.float64, generator=g) * cdf[-1])
+        tok = torch.randperm(V, device="cuda", generator=g)[ranks].to(torch.int32)
+        W = torch.randn(V, d, device="cuda", generator=g)
+        dx = torch.randn(n, d, device="cuda", generator=g).bfloat16()
+        for _ in range(a.reps):
+            dgx.embed_fwd(tok, W, scale=32.0, out_dtype=torch.bfloat16)
+            dgx.embed_bwd(tok, dx, V, scale=32.0)
     elif a.kind == "gemm_f32":
         A, B, dC = (torch.randn(a.n, a.n, device="cuda", generator=g) for _ in range(3))
         for _ in range(a.reps):

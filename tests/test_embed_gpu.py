@@ -57,7 +57,7 @@ def test_forward(dgx, n, V, d, w, x, S):
 
 
 @pytest.mark.parametrize("n,V,d", [(1, 1, 1), (1, 1000, 1024), (7, 13, 5), (300, 65, 384), (257, 5000, 33),
-                                   (128, 500, 264), (129, 500, 264), (5000, 77, 130), (64, 300, 2050), (20000, 700, 256), (33, 140000, 64),
+                                   (128, 500, 264), (129, 500, 264), (5000, 77, 130), (64, 300, 2050), (20000, 700, 256), (33, 140000, 64), (100, 70000, 136),
                                    (70000, 3, 40)])
 @pytest.mark.parametrize("kind", ["spread", "one", "hot", "invalid", "none"])
 @pytest.mark.parametrize("gx,w", [("f32", "f32"), ("f32", "bf16"), ("bf16", "f32"), ("bf16", "bf16")])

@@ -11,7 +11,7 @@ namespace dgx {
 
 constexpr int kHeadMaxK = 256;          // teacher entries per row
 constexpr int kHeadSlot = 64;          // columns per entry of a target list's start table
-constexpr int kHeadMaxRows = 1 << 23;   // rows, and columns of the vocabulary: tile counts fit 32 bits
+constexpr int kHeadMaxDim = 1 << 23;    // R, V and d: tile and fragment counts fit 32 bits
 
 // One problem: logits z = (H . W^T + bias) / T of R rows over V columns, and a
 // sparse target per row: K ids with K probabilities. The hard target is K = 1

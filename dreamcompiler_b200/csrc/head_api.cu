@@ -3,6 +3,7 @@
 // target (dgx_linear_nll_*) and for a teacher's largest logits
 // (dgx_linear_distill_*). Argument checks and workspace handling; the work is
 // in head.cu.
+#include <algorithm>
 #include <cmath>
 
 #include "common.h"
@@ -14,8 +15,8 @@ namespace {
 
 dgx_status head_check(const char* op, const void* H, int ldh, const void* W, int ldw, int R, int V, int d, int K) {
   if (R < 0 || V <= 0 || d <= 0) return set_error(DGX_EINVAL, "%s: bad size R=%d V=%d d=%d", op, R, V, d);
-  if (R > kHeadMaxRows || V > kHeadMaxRows)
-    return set_error(DGX_EINVAL, "%s: R=%d or V=%d above %d", op, R, V, kHeadMaxRows);
+  if (R > kHeadMaxDim || V > kHeadMaxDim || d > kHeadMaxDim)
+    return set_error(DGX_EINVAL, "%s: R=%d, V=%d or d=%d above %d", op, R, V, d, kHeadMaxDim);
   if (K < 1 || K > kHeadMaxK) return set_error(DGX_EINVAL, "%s: K=%d (1..%d entries per row)", op, K, kHeadMaxK);
   if (ldh < d || ldw < d || ldh % 8 || ldw % 8)
     return set_error(DGX_EINVAL, "%s: row pitch ldh=%d ldw=%d (>= d=%d and a multiple of 8)", op, ldh, ldw, d);
@@ -94,12 +95,12 @@ dgx_status check_temperature(const char* op, float t) {
 extern "C" {
 
 size_t dgx_linear_nll_workspace_size(int R, int V, int d, int backward) {
-  if (R <= 0 || V <= 0 || d <= 0) return 0;
+  if (R <= 0 || V <= 0 || d <= 0 || std::max({R, V, d}) > kHeadMaxDim) return 0;
   return backward ? head_bwd_scratch_bytes(R, V, d, 1, false) : head_fwd_scratch_bytes(R, V, d, 1, false);
 }
 
 size_t dgx_linear_distill_workspace_size(int R, int V, int d, int K, int backward) {
-  if (R <= 0 || V <= 0 || d <= 0 || K < 1 || K > kHeadMaxK) return 0;
+  if (R <= 0 || V <= 0 || d <= 0 || std::max({R, V, d}) > kHeadMaxDim || K < 1 || K > kHeadMaxK) return 0;
   return backward ? head_bwd_scratch_bytes(R, V, d, K, true) : head_fwd_scratch_bytes(R, V, d, K, true);
 }
 

@@ -165,7 +165,7 @@ int small_smem(int R, int d) { return (d + 31) / 32 * ((R + 7) / 8) * 512; }
 }  // namespace
 
 // Statistics slots (blocks) of the small kernel, 0 where it does not apply: up
-// to 32 rows whose fragments fit 96 KB of shared memory (two blocks per SM).
+// to 16 rows whose fragments fit 96 KB of shared memory (two blocks per SM).
 int head_small_slots(int R, int V, int d) {
   if (R > 16 || small_smem(R, d) > 96 * 1024) return 0;
   const int tiles = (V + kTileRows - 1) / kTileRows;

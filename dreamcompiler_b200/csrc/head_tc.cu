@@ -421,7 +421,7 @@ cudaError_t head_logits_tc(HeadTcArgs a, const void* H, int ldh, const void* W, 
   // in L2 while the W tiles stream by: W is read from HBM once per group
   // (groups of 8 read it four times at R = 8192: 8192 x 65536 x 2048 training
   // 6.74 -> 6.58 ms, 4096 x 32768 x 1024 874 -> 863 us with one group).
-  a.group_m = (int)std::max<long long>(8, (48ll << 20) / (2ll * HD_BM * 2 * a.d));
+  a.group_m = (int)std::min<long long>(a.tiles_m, std::max<long long>(8, (48ll << 20) / (2ll * HD_BM * 2 * a.d)));
   const int pairs = (int)std::min<long long>((long long)a.tiles_m * a.tiles_n, num_sms() / 2);
   auto run = [&](auto mode, auto bias, auto warps) {
     constexpr int M = decltype(mode)::value, EW = decltype(warps)::value;

@@ -406,9 +406,10 @@ dgx_status dgx_heads_to_rows(const void* src, void* dst, int ld, int col0, int B
  * products (scale is applied after them, in fp32); db is summed unrounded.
  * accumulate: DGX_ACC_W adds to dW (fp32) and db, DGX_ACC_H to dH (fp32), so
  * that several losses, heads or micro-batches sum into one gradient. Every
- * result is the same bits on every run. workspace: dgx_linear_*_workspace_size() bytes, 128-byte aligned,
- * or NULL for the library's own buffer; its contents need not survive between
- * calls. Rows of H must be finite even where the row has no target (0 * inf in
+ * result is the same bits on every run. R, V and d are at most 2^23.
+ * workspace: dgx_linear_*_workspace_size() bytes, 128-byte aligned, or NULL
+ * for the library's own buffer; its contents need not survive between calls.
+ * Rows of H must be finite even where the row has no target (0 * inf in
  * dW); a row without a target has loss 0 and dH 0.
  *
  * dgx_linear_nll_*: loss_r = lse_r - z_{r,target[r]}; a target outside [0, V)
@@ -460,8 +461,8 @@ dgx_status dgx_embed_fwd(const int* tok, const void* W, dgx_dtype w_type, int ld
  * often), rounded once, the same bits on every run. accumulate = 0 writes
  * every row of dW (zero where the token does not occur); accumulate = 1 (fp32
  * dW) adds to the rows of the tokens that occur and leaves the others alone.
- * workspace: dgx_embed_bwd_workspace_size() bytes, 16-byte aligned, or NULL
- * for the library's own buffer.
+ * workspace: dgx_embed_bwd_workspace_size() bytes (0 where few tokens need
+ * none), 16-byte aligned, or NULL for the library's own buffer.
  * dgx_embedding_bwd (runtime/ops/autograd.inc:330-341) adds with fp32 atomics.
  */
 dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int lddx, float scale, void* dW,

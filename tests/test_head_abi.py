@@ -47,6 +47,16 @@ def test_head_backward_refusals(lib):
     assert nll_bwd(lib, dH=None, dW=None) == L.DGX_OK  # nothing asked for
 
 
+def test_head_dimension_limit(lib):
+    from dreamcompiler_b200 import _lib as L
+    top = 1 << 23
+    for kw in (dict(R=top + 1), dict(V=top + 1), dict(d=top + 8, ldh=top + 8, ldw=top + 8)):
+        assert nll_fwd(lib, **kw) == L.DGX_EINVAL, kw
+        assert b"above" in lib.dgx_last_error()
+    assert lib.dgx_linear_nll_workspace_size(4, 10, top + 1, 0) == 0
+    assert lib.dgx_linear_distill_workspace_size(4, 10, 64, 4, 1) > 0
+
+
 def test_distill_refusals(lib):
     from dreamcompiler_b200 import _lib as L
 

@@ -127,7 +127,8 @@ __global__ void __launch_bounds__(128) head_lists_kernel(const int* __restrict__
 
 // ---------------------------------------------------------------- forward
 // lse and loss from the statistics part[slot][R] (max of the raw logits and
-// sum of exp((z - max) / T) over the slot's columns). A block owns 32 rows, one
+// sum of exp((z - max) / T) over the slot's columns; without a hard target's
+// column, which nll_row adds). A block owns 32 rows, one
 // per lane; its NW warps walk the slots, eight loads in flight, and their
 // results are joined in warp order. Hard target: sq == null.
 template <int NW>
@@ -165,16 +166,17 @@ __global__ void __launch_bounds__(NW * 32) head_finish_kernel(
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < NW; ++i) s += ms[i][lane].y * expf((ms[i][lane].x - base) * inv_t);
-    const float log_s = logf(s);
-    if (row < R) lse[row] = base * inv_t + log_s;
     if (!sq) {
-      // z - lse = (raw - max)/T - log s: subtracting the maximum first keeps
-      // the loss accurate when the logits are large
       if (row < R) {
         const int id = sid[row];
-        loss[row] = id >= 0 && id < V ? log_s - (zs[row] - base) * inv_t : 0.f;
+        const bool has = id >= 0 && id < V;
+        nll_row(m, s, has ? zs[row] : 0.f, has, inv_t, loss[row], lse[row]);
       }
     } else {
+      // z - lse = (raw - max)/T - log s: subtracting the maximum first keeps
+      // the loss accurate when the logits are large
+      const float log_s = logf(s);
+      if (row < R) lse[row] = base * inv_t + log_s;
       base_s[lane] = base;
       logs_s[lane] = log_s;
     }

@@ -51,6 +51,7 @@ struct HeadTcArgs {
   const uint16_t* start;    // [R][slots] first entry with id >= kHeadSlot * slot, or null (K = 1)
   int slots;
   float* zs;                // [R][K] out: raw logits at the ids (statistics)
+                            // (a hard target's is left out of the row's statistics)
   float2* part;             // [ceil(n / head_stat_cols())][R] out: (max, sum) per slot of columns (statistics)
   const float* live;        // [R] 0 where the row has no target, or null (id in [0, V))
   const float* dloss;       // [R] or null
@@ -94,5 +95,29 @@ size_t head_fwd_scratch_bytes(int R, int V, int d, int K, bool lists);
 size_t head_bwd_scratch_bytes(int R, int V, int d, int K, bool lists);
 dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s);
 dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s);
+
+// lse and loss of one row with a hard target, from the statistics (m, s) of the
+// OTHER columns (max of the raw logits, sum of exp((z - m) / T)) and the
+// target's raw logit zt (has = false: the row has none, (m, s) are all columns).
+// With the target left out of the sum a small loss, log(1 + sum / exp(zt)),
+// keeps its relative precision; log of a sum near 1 would lose it.
+__device__ __forceinline__ void nll_row(float m, float s, float zt, bool has, float inv_t, float& loss, float& lse) {
+  loss = 0.f;
+  const float mx = has ? fmaxf(m, zt) : m;
+  if (!has || isinf(mx)) {  // every column masked, or an overflow: loss NaN or inf as inf - inf gives it
+    lse = mx * inv_t + logf(s);
+    if (has) loss = lse - zt * inv_t;
+    return;
+  }
+  const float delta = (m - zt) * inv_t;
+  if (delta <= 0.f) {
+    loss = log1pf(s * expf(delta));
+    lse = zt * inv_t + loss;
+  } else {
+    const float log_s = logf(s + expf(-delta));
+    loss = delta + log_s;
+    lse = m * inv_t + log_s;
+  }
+}
 
 }  // namespace dgx

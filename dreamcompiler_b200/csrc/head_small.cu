@@ -58,7 +58,7 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 }
 
 // NT: groups of 8 rows of H. part[block][R] gets the statistics of the block's
-// columns, zs[r] the target's logit; a single block holds all columns and writes
+// columns but the target's, zs[r] the target's logit; a single block holds all columns and writes
 // loss and lse itself.
 template <int NT>
 __global__ void __launch_bounds__(kWarps * 32) head_small_kernel(const __nv_bfloat16* __restrict__ H, int ldh,
@@ -125,8 +125,14 @@ __global__ void __launch_bounds__(kWarps * 32) head_small_kernel(const __nv_bflo
         if (v0 >= V) z0 = -INFINITY;
         if (v1 >= V) z1 = -INFINITY;
         const int id = tg[nt][k];
-        if (id == v0 && v0 < V) zs[nt * 8 + 2 * t + k] = z0;
-        if (id == v1 && v1 < V) zs[nt * 8 + 2 * t + k] = z1;
+        if (id == v0 && v0 < V) {
+          zs[nt * 8 + 2 * t + k] = z0;
+          z0 = -INFINITY;
+        }
+        if (id == v1 && v1 < V) {
+          zs[nt * 8 + 2 * t + k] = z1;
+          z1 = -INFINITY;
+        }
         const float mn = max3f(m[nt][k], z0, z1), base = mn == -INFINITY ? 0.f : mn;
         s[nt][k] = s[nt][k] * ex2((m[nt][k] - base) * kLog2e) + (ex2((z0 - base) * kLog2e) + ex2((z1 - base) * kLog2e));
         m[nt][k] = mn;
@@ -152,10 +158,9 @@ __global__ void __launch_bounds__(kWarps * 32) head_small_kernel(const __nv_bflo
       part[(size_t)blockIdx.x * R + threadIdx.x] = make_float2(mm, ss);
     } else {
       const int id = target[threadIdx.x];
-      const float base = mm == -INFINITY ? 0.f : mm, log_s = logf(ss);
-      lse[threadIdx.x] = base + log_s;
+      const bool has = id >= 0 && id < V;
       // zs[row] was written by this block before the barrier
-      loss[threadIdx.x] = id >= 0 && id < V ? log_s - (__ldcg(zs + threadIdx.x) - base) : 0.f;
+      nll_row(mm, ss, has ? __ldcg(zs + threadIdx.x) : 0.f, has, 1.f, loss[threadIdx.x], lse[threadIdx.x]);
     }
   }
 }

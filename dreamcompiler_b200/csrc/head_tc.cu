@@ -105,6 +105,10 @@ __device__ __forceinline__ void stats32(float (&z)[32], int n0, int j0, int row,
     float v = 0.f;
 #pragma unroll
     for (int j = 0; j < 32; ++j) v = at == j ? z[j] : v;
+    if (!a.sq) {  // a hard target stays out of the sum
+#pragma unroll
+      for (int j = 0; j < 32; ++j) z[j] = at == j ? -INFINITY : z[j];
+    }
     if ((unsigned)at < 32u) {
       a.zs[(size_t)row * a.K + tg.k] = v;
       tg.next();

@@ -295,6 +295,50 @@ def test_non_finite_rows_stay_in_their_rows(dgx):
     assert not torch.isfinite(loss[alive])
 
 
+@pytest.mark.parametrize("R,V,d,bias", [(1, 65, 64, False), (12, 1000, 64, True), (40, 65, 64, True),
+                                        (300, 1000, 1024, False)])
+def test_small_losses_keep_their_relative_precision(dgx, R, V, d, bias):
+    """A target far above every other column: the loss is log(1 + a small sum), which log of the whole sum would
+    round to multiples of 2^-23. All logits are exact (multiples of 1/8), so what is left is the exponentials:
+    arguments up to 30 log2(e) < 44 rounded twice (44 * 2^-23), the exponential (2^-21), at most 64 additions in a
+    row (64 * 2^-24), log1p and expf (a few 2^-23): below 1.2e-5 of the loss."""
+    H = torch.zeros(R, d, device="cuda", dtype=torch.bfloat16)
+    H[:, 0] = 1
+    W = torch.zeros(V, d, device="cuda", dtype=torch.bfloat16)
+    W[:, 0] = -(torch.arange(V, device="cuda") % 9) / 8
+    target = (torch.arange(R, device="cuda", dtype=torch.int32) * 7) % V
+    rows = torch.arange(R, device="cuda")
+    H[rows, 1 + rows] = 1  # column 1 + r lifts row r's target only
+    W[target.long(), 1 + rows] = (12 + rows % 8 * 2).to(W.dtype)
+    b = None
+    if bias:
+        b = torch.arange(V, device="cuda", dtype=torch.float32) % 3 / 4
+    z = H.to(F64) @ W.to(F64).T + (0 if b is None else b.to(F64))
+    zt = z.gather(1, target.long()[:, None])
+    others = torch.exp(z - zt).scatter(1, target.long()[:, None], 0.0).sum(1)
+    want = torch.log1p(others)
+    loss, lse = dgx.linear_nll_fwd(H, W, target, bias=b)[:2]
+    assert float(want.max()) < 0.05
+    within(loss, want, 1.2e-5 * want, "loss")
+    within(lse, zt[:, 0] + want, 2 ** -22 * (zt[:, 0].abs() + want + 1), "lse")
+
+
+@pytest.mark.parametrize("R", [3, 200])
+def test_rows_masked_in_every_column(dgx, R):
+    """No distribution: lse is -inf and the loss NaN where a target is asked for, as inf - inf; a masked target
+    alone has loss inf; the rows beside them are not touched."""
+    H = torch.ones(R, 64, device="cuda", dtype=torch.bfloat16)
+    W = torch.ones(10, 64, device="cuda", dtype=torch.bfloat16)
+    t = torch.full((R,), 4, device="cuda", dtype=torch.int32)
+    t[1] = -1
+    b = torch.full((10,), float("-inf"), device="cuda")
+    loss, lse = dgx.linear_nll_fwd(H, W, t, bias=b)[:2]
+    assert torch.isneginf(lse).all() and loss[1] == 0 and torch.isnan(loss[0]) and torch.isnan(loss[2:]).all()
+    b[:3] = 0
+    loss, lse = dgx.linear_nll_fwd(H, W, t, bias=b)[:2]
+    assert torch.isfinite(lse).all() and loss[1] == 0 and torch.isposinf(loss[0]) and torch.isposinf(loss[2:]).all()
+
+
 def test_large_logits(dgx):
     """Logits of several thousand: the softmax neither overflows nor loses the
     loss of the leading id."""

@@ -453,14 +453,18 @@ __device__ __forceinline__ int search(const SumArgs& a, int lo, int hi, int at, 
 // Writes the block's part of token t and notes the token if that was the last part.
 __device__ __forceinline__ void put_part(const SumArgs& a, SumShared& sh, int blk, int slab, int side, int t, int lane,
                                          const float (&acc)[8]) {
+  // the token's blocks: from the one it runs out of (its last position's
+  // token) to the last one whose first position has it; the 32 neighbours on
+  // either side first (one round trip), then a search
+  const bool fwd = blk + 1 + lane < a.blocks && a.sorted[(size_t)(blk + 1 + lane) * kBlockPos].x == t;
+  const bool back = !side && lane < blk && a.sorted[(size_t)(blk - lane) * kBlockPos - 1].x == t;
   float* p = a.parts + ((size_t)blk * 2 + side) * a.slabs * kSlab + slab * kSlab;
 #pragma unroll
   for (int k = 0; k < 8; ++k) p[lane + 32 * k] = acc[k];
   __threadfence();
-  // the token's blocks: from the one it runs out of (its last position's
-  // token) to the last one whose first position has it
-  const int b0 = side ? blk : search(a, 0, blk, kBlockPos - 1, t, lane);
-  const int b1 = search(a, blk + 1, a.blocks, 0, t + 1, lane) - 1;
+  const int nf = __popc(__ballot_sync(0xffffffffu, fwd)), nb = __popc(__ballot_sync(0xffffffffu, back));
+  const int b0 = nb < 32 ? blk - nb : search(a, 0, blk - 32, kBlockPos - 1, t, lane);
+  const int b1 = nf < 32 ? blk + nf : search(a, blk + 33, a.blocks, 0, t + 1, lane) - 1;
   __syncwarp();
   if (lane == 0 && atomicAdd(&a.counters[(size_t)b0 * a.slabs + slab], 1) == b1 - b0) {
     sh.last_token[side] = t;

@@ -75,6 +75,22 @@ def test_backward(dgx, n, V, d, kind, gx, w):
     assert torch.equal(got, dgx.embed_bwd(tok, dx, V, scale=scale, out_dtype=DT[w]))
 
 
+@pytest.mark.parametrize("before", [0, 1, 127, 128, 33 * 128 + 5])
+@pytest.mark.parametrize("span", [1, 128, 129, 31 * 128, 32 * 128 + 1, 33 * 128, 33 * 128 + 1, 65 * 128 - 1])
+@pytest.mark.parametrize("after", [0, 40 * 128 + 3])
+def test_backward_of_a_token_over_many_blocks(dgx, before, span, after):
+    """One id whose sorted run starts and ends at, before and after the edges of the summing blocks."""
+    g = torch.Generator(device="cuda").manual_seed(before + span + after)
+    n, V, d = before + span + after, 3, 16
+    tok = torch.tensor([0] * before + [1] * span + [2] * after, dtype=torch.int32, device="cuda")
+    tok = tok[torch.randperm(n, device="cuda", generator=g)].contiguous()
+    dx = torch.randn(n, d, device="cuda", generator=g)
+    got = dgx.embed_bwd(tok, dx, V)
+    ref, mag, cnt = truth(tok, dx, V, 1.0)
+    tol = U * (cnt[:, None] + 2) * mag + U * ref.abs()
+    assert ((got.to(F64) - ref).abs() <= tol).all()
+
+
 def truth(tok, dx, V, scale):
     s32 = float(torch.tensor(scale, dtype=torch.float32))
     ok = (tok >= 0) & (tok < V)

@@ -388,11 +388,16 @@ dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s) {
   t.part = c.take<float2>((size_t)slots * a.R);
   t.zs = c.take<float>((size_t)a.R * a.K);
   t.n = a.V;
+  const bool whole = !a.teacher && !small && a.V <= 256;  // one tile holds a row: finished in the tile's epilogue
+  if (whole) {
+    t.loss = a.loss;
+    t.lse_out = a.lse;
+  }
   cudaError_t e = target_lists(a, c, t, s);
   if (e == cudaSuccess)
     e = small ? head_small(t, a.H, a.ldh, a.W, a.ldw, small, a.loss, a.lse, s)
               : head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, false, nullptr, 0, s);
-  if (e == cudaSuccess && small != 1) {
+  if (e == cudaSuccess && small != 1 && !whole) {
     // few slots: few warps, so that many rows do not pay for idle ones
     const bool wide = slots > 32;
     e = launch_dependent(wide ? head_finish_kernel<32> : head_finish_kernel<4>, (a.R + 31) / 32, wide ? 1024 : 128, 0, 1,

@@ -53,6 +53,8 @@ struct HeadTcArgs {
   float* zs;                // [R][K] out: raw logits at the ids (statistics)
                             // (a hard target's is left out of the row's statistics)
   float2* part;             // [ceil(n / head_stat_cols())][R] out: (max, sum) per slot of columns (statistics)
+  float *loss, *lse_out;    // [R] out: a hard target's results where one tile holds every column
+                            // (n = V <= 256; zs and part are not written then), or null (statistics)
   const float* live;        // [R] 0 where the row has no target, or null (id in [0, V))
   const float* dloss;       // [R] or null
   const float* lse;         // [R]

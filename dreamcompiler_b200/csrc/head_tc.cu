@@ -31,14 +31,16 @@ constexpr uint32_t HD_TMEM_COLS = 512;
 constexpr int kStats = 0, kGrad = 1;
 // EW epilogue warps; a TMEM lane quarter's 256 columns are split over the
 // quarter's warps. After the operand stages: a 4 KB staging box for G per
-// warp (the gradient), and each warp's columns of the bias.
+// warp (the gradient), each warp's columns of the bias, and its rows' results
+// of a tile (statistics; twice, for alternate tiles).
 template <int MODE, bool BIAS, int EW>
 struct HdCfg {
   static constexpr int COLS = 4 * HD_BN / EW;
   static constexpr int THREADS = 64 + 32 * EW;
   static constexpr int OUT = MODE == kGrad ? EW * 4096 : 0;
   static constexpr int BIAS_BYTES = BIAS ? 4 * HD_BN * 4 : 0;
-  static constexpr int TAIL = OUT + BIAS_BYTES + 1024 + 256;
+  static constexpr int ROWS = MODE == kStats ? 2 * EW * 32 * 3 * 4 : 0;
+  static constexpr int TAIL = OUT + BIAS_BYTES + ROWS + 1024 + 256;
   static constexpr int FIT = (232448 - TAIL) / HD_STAGE;
   static constexpr int STAGES = FIT < 6 ? FIT : 6;
   static constexpr int SMEM = STAGES * HD_STAGE + TAIL;
@@ -91,10 +93,10 @@ struct Target {
   }
 };
 
-// Row statistics of 32 logits of one row: the target's logits to zs, the
-// running maximum and sum. n0: column within the piece, j0: its vocabulary id.
+// Row statistics of 32 logits of one row: the target's logits to zs (or zt),
+// the running maximum and sum. n0: column within the piece, j0: its vocabulary id.
 __device__ __forceinline__ void stats32(float (&z)[32], int n0, int j0, int row, const HeadTcArgs& a, Target& tg,
-                                        float& m, float& s) {
+                                        float& m, float& s, float& zt) {
   if (n0 + 32 > a.n) {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
@@ -110,7 +112,8 @@ __device__ __forceinline__ void stats32(float (&z)[32], int n0, int j0, int row,
       for (int j = 0; j < 32; ++j) z[j] = at == j ? -INFINITY : z[j];
     }
     if ((unsigned)at < 32u) {
-      a.zs[(size_t)row * a.K + tg.k] = v;
+      zt = v;
+      if (!a.loss) a.zs[(size_t)row * a.K + tg.k] = v;
       tg.next();
     }
   }
@@ -181,7 +184,7 @@ __global__ void __launch_bounds__(64 + 32 * HD_EPI_WARPS, 1)
   constexpr int COLS = Cfg::COLS;
   constexpr int HD_STAGES = Cfg::STAGES;
   uint8_t* out_stage = smem + HD_STAGES * HD_STAGE;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_stage + Cfg::OUT + Cfg::BIAS_BYTES);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_stage + Cfg::OUT + Cfg::BIAS_BYTES + Cfg::ROWS);
   uint64_t* empty_bar = full_bar + HD_STAGES;
   uint64_t* accf_bar = empty_bar + HD_STAGES;  // [2]
   uint64_t* acce_bar = accf_bar + 2;           // [2]
@@ -219,7 +222,7 @@ __global__ void __launch_bounds__(64 + 32 * HD_EPI_WARPS, 1)
   cluster_sync_all2();  // both CTAs' barriers are initialised before any cross-CTA traffic
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (MODE == kGrad || !a.loss) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // not the last kernel
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const int num_tiles = a.tiles_m * a.tiles_n;
@@ -294,6 +297,8 @@ __global__ void __launch_bounds__(64 + 32 * HD_EPI_WARPS, 1)
     const int part = (warp - 2) >> 2;    // its columns of the tile
     uint8_t* st = out_stage + (warp - 2) * 4096;
     float* bias_s = reinterpret_cast<float*>(out_stage + Cfg::OUT) + (warp - 2) * COLS;
+    float* rows_s = reinterpret_cast<float*>(out_stage + Cfg::OUT + Cfg::BIAS_BYTES);
+    const bool whole = MODE == kStats && a.loss;  // this tile finishes its rows
     uint32_t issued = 0, use = 0;
     for (int t = pair; t < num_tiles; t += npairs, ++use) {
       const int buf = use & 1;
@@ -323,12 +328,14 @@ __global__ void __launch_bounds__(64 + 32 * HD_EPI_WARPS, 1)
         for (int j = lane; j < COLS; j += 32) bias_s[j] = nbase + j < a.n ? __ldg(a.bias + a.c0 + nbase + j) : 0.f;
         __syncwarp();
       }
-      if (!mbar_wait(&accf_bar[buf], (use >> 1) & 1, wc)) break;
+      // where the quarter's warps meet below, one that gave up still comes
+      const bool ok = mbar_wait(&accf_bar[buf], (use >> 1) & 1, wc);
+      if (!ok && !whole) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + buf * HD_BN + part * COLS;
-      float m = -INFINITY, s = 0.f;
+      float m = -INFINITY, s = 0.f, zt = 0.f;
 #pragma unroll 1
-      for (int c = 0; c < COLS; c += 32) {
+      for (int c = ok ? 0 : COLS; c < COLS; c += 32) {
         float z[32];
         {
           uint32_t r[32];
@@ -361,7 +368,7 @@ __global__ void __launch_bounds__(64 + 32 * HD_EPI_WARPS, 1)
           }
         }
         if constexpr (MODE == kStats) {
-          stats32(z, n0, j0, row, a, tg, m, s);
+          stats32(z, n0, j0, row, a, tg, m, s, zt);
         } else {
           grad32(z, j0, a, tg, w, lse);
           // 64 columns to a box; a half past the piece is not stored
@@ -389,7 +396,25 @@ __global__ void __launch_bounds__(64 + 32 * HD_EPI_WARPS, 1)
           }
         }
       }
-      if (MODE == kStats && row_ok && nbase < a.n) a.part[(size_t)(nbase / COLS) * a.R + row] = make_float2(m, s);
+      if (whole) {
+        float* mine = rows_s + ((buf * HD_EPI_WARPS + warp - 2) * 32 + lane) * 3;
+        mine[0] = m;
+        mine[1] = s;
+        mine[2] = zt;
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "n"(8 * HD_EPI_WARPS) : "memory");
+        if (part == 0 && row_ok) {  // joins the quarter's warps in column order
+          constexpr int NEXT = 4 * 32 * 3;
+#pragma unroll
+          for (int i = 1; i < HD_EPI_WARPS / 4; ++i) m = fmaxf(m, mine[i * NEXT]);
+          const float base = m == -INFINITY ? 0.f : m;
+          s = 0.f;
+#pragma unroll
+          for (int i = 0; i < HD_EPI_WARPS / 4; ++i) s += mine[i * NEXT + 1] * expf((mine[i * NEXT] - base) * a.inv_t);
+          const int id = a.sid[row];
+          const bool has = id >= 0 && id < a.V;
+          nll_row(m, s, has ? mine[id / COLS * NEXT + 2] : 0.f, has, a.inv_t, a.loss[row], a.lse_out[row]);
+        }
+      } else if (MODE == kStats && row_ok && nbase < a.n) a.part[(size_t)(nbase / COLS) * a.R + row] = make_float2(m, s);
     }
     if (MODE == kGrad && lane == 0) bulk_wait0();
   }

@@ -295,6 +295,19 @@ def test_non_finite_rows_stay_in_their_rows(dgx):
     assert not torch.isfinite(loss[alive])
 
 
+@pytest.mark.parametrize("R,V,d", [(17, 1, 8), (300, 256, 1000), (700, 129, 64), (60000, 65, 24), (513, 250, 770)])
+@pytest.mark.parametrize("bias", [None, "masked"])
+def test_nll_vocabulary_of_one_tile(dgx, R, V, d, bias):
+    """Up to 256 columns: loss and lse leave the logits kernel itself (60000 rows: several tiles per SM pair)."""
+    p = Problem(R, V, d, bias=bias, ignored=0.2, weighted=True, seed=R + V, scale=1.0 / R)
+    mean = torch.full((1,), float("nan"), device="cuda")
+    loss, lse = p.fwd(dgx, mean=mean)
+    p.check_fwd(loss, lse)
+    within(mean, p.loss.mean()[None], p.tol_loss.mean()[None] + 2 ** -18 * p.loss.abs().mean(), "mean")
+    p.check_bwd(*p.bwd(dgx, lse))
+    dgx.sync_check()
+
+
 @pytest.mark.parametrize("R,V,d,bias", [(1, 65, 64, False), (12, 1000, 64, True), (40, 65, 64, True),
                                         (300, 1000, 1024, False)])
 def test_small_losses_keep_their_relative_precision(dgx, R, V, d, bias):

@@ -10,7 +10,8 @@
 //
 // Both run the main loop of gemm2_kernel (TMA operand ring, one MMA-issuing
 // thread in the leader, two TMEM accumulators) with eight or sixteen epilogue
-// warps.
+// warps. Bound by the tensor pipe from d = 1024 on (4096 x 32768 x 1024: 170 us
+// and 175 us, 1.61 and 1.57 PFLOP/s), by the epilogue for short contractions.
 #include <algorithm>
 
 #include "gemm.h"

@@ -252,7 +252,7 @@ def _ws(workspace: Optional[torch.Tensor]):
     return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
 
 
-def _head_check(H, W, bias, rows32, rowsf):
+def _head_check(H, W, bias, rows32, rowsf, mean=None):
     """Shapes and types shared by the vocabulary-head wrappers; returns (R, V,
     d) and the row pitches of H and W. Each attribute of a tensor is asked for
     once: for a few rows these checks weigh as much as the kernels."""
@@ -268,6 +268,8 @@ def _head_check(H, W, bias, rows32, rowsf):
     for t in rowsf:
         if t is not None:
             assert t.get_device() == dev and t.dtype is torch.float32 and t.is_contiguous() and t.shape[0] == R
+    if mean is not None:
+        assert mean.get_device() == dev and mean.dtype is torch.float32 and mean.numel() == 1, "mean: one fp32 element"
     # torch reports any stride for a single row
     return R, V, d, ldh if R > 1 else (d + 7) // 8 * 8, ldw if V > 1 else (d + 7) // 8 * 8
 
@@ -294,7 +296,7 @@ def linear_nll_fwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, *, bi
     int32 (outside [0, V): no target, loss 0). Returns (loss [R], lse [R]), the
     row log-sum-exp being what linear_nll_bwd needs; `mean` (one fp32 element)
     receives sum(loss) / R."""
-    R, V, d, ldh, ldw = _head_check(H, W, bias, target, (loss, lse))
+    R, V, d, ldh, ldw = _head_check(H, W, bias, target, (loss, lse), mean)
     assert target.dim() == 1
     if loss is None:
         loss = torch.empty(R, device=H.device, dtype=torch.float32)
@@ -350,7 +352,7 @@ def linear_distill_fwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teac
     against a teacher's K largest logits per row: idx [R, K] int32 vocabulary
     ids (outside [0, V): absent), teacher [R, K] fp32. Returns (loss [R],
     lse [R]) with lse the log-sum-exp of the student's logits / T."""
-    R, V, d, ldh, ldw = _head_check(H, W, bias, idx, (teacher, loss, lse))
+    R, V, d, ldh, ldw = _head_check(H, W, bias, idx, (teacher, loss, lse), mean)
     assert idx.dim() == 2 and teacher.shape == idx.shape
     if loss is None:
         loss = torch.empty(R, device=H.device, dtype=torch.float32)

@@ -460,3 +460,15 @@ def test_refusals(dgx):
         with pytest.raises(AssertionError):
             wrong()
     dgx.sync_check()
+
+
+def test_mean_must_be_one_float_on_the_device(dgx):
+    H = torch.zeros(8, 64, device="cuda", dtype=torch.bfloat16)
+    W = torch.zeros(100, 64, device="cuda", dtype=torch.bfloat16)
+    t = torch.zeros(8, device="cuda", dtype=torch.int32)
+    for bad in (torch.zeros(1), torch.zeros(1, device="cuda", dtype=torch.bfloat16), torch.zeros(0, device="cuda"),
+                torch.zeros(2, device="cuda")):
+        with pytest.raises(AssertionError, match="mean"):
+            dgx.linear_nll_fwd(H, W, t, mean=bad)
+        with pytest.raises(AssertionError, match="mean"):
+            dgx.linear_distill_fwd(H, W, t[:, None], torch.zeros(8, 1, device="cuda"), mean=bad)

@@ -662,6 +662,10 @@ bool vec_ok(const void* p, int type, int ld, int d) {
 
 size_t align16(size_t b) { return (b + 15) & ~size_t(15); }
 
+// Tokens of one gradient call. The sort and the sums count positions in 32
+// bits and step past the last one by up to a cluster's stride (16 x 1024).
+constexpr int kMaxTokens = 0x7fffffff - 0xffff;
+
 struct Layout {
   bool few;           // the one-launch form (by the table's fp32 size, whatever its type)
   int blocks, slabs;  // blocks of kBlockPos positions
@@ -780,7 +784,7 @@ dgx_status dgx_embed_fwd(const int* tok, const void* W, dgx_dtype w_type, int ld
 }
 
 size_t dgx_embed_bwd_workspace_size(int n, int d, int V) {
-  if (n <= 0 || d <= 0 || V <= 0) return 0;
+  if (n <= 0 || n > kMaxTokens || d <= 0 || V <= 0) return 0;
   return layout(n, d, V).bytes;
 }
 
@@ -790,6 +794,7 @@ dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int 
   DGX_FAULT_POINT("dgx_embed_bwd");
   if (n < 0 || d <= 0 || V <= 0 || V == 0x7fffffff)
     return set_error(DGX_EINVAL, "dgx_embed_bwd: bad size n=%d d=%d V=%d", n, d, V);
+  if (n > kMaxTokens) return set_error(DGX_EINVAL, "dgx_embed_bwd: n=%d above %d", n, kMaxTokens);
   if (!type_ok(dx_type) || !type_ok(dw_type))
     return set_error(DGX_EINVAL, "dgx_embed_bwd: types %d %d", dx_type, dw_type);
   if (lddx < d || lddw < d) return set_error(DGX_EINVAL, "dgx_embed_bwd: row pitch %d or %d < d=%d", lddx, lddw, d);

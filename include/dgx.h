@@ -461,6 +461,7 @@ dgx_status dgx_embed_fwd(const int* tok, const void* W, dgx_dtype w_type, int ld
  * often), rounded once, the same bits on every run. accumulate = 0 writes
  * every row of dW (zero where the token does not occur); accumulate = 1 (fp32
  * dW) adds to the rows of the tokens that occur and leaves the others alone.
+ * n is at most 2^31 - 65536.
  * workspace: dgx_embed_bwd_workspace_size() bytes (0 where few tokens need
  * none), 16-byte aligned, or NULL for the library's own buffer.
  * dgx_embedding_bwd (runtime/ops/autograd.inc:330-341) adds with fp32 atomics.

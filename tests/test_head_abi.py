@@ -94,6 +94,22 @@ def test_embed_refusals(lib):
     assert fwd(n=0, tok=None, x=None) == L.DGX_OK
 
 
+def test_embed_token_limit(lib):
+    """Positions are counted in 32 bits and stepped past the last one: a count that would wrap is refused before
+    anything runs (the last accepted one gets as far as the workspace check)."""
+    from dreamcompiler_b200 import _lib as L
+    top = (1 << 31) - (1 << 16)
+
+    def bwd(n):
+        return lib.dgx_embed_bwd(FAKE, FAKE, 0, 16, 1.0, FAKE, 0, 16, n, 16, 10, 0, FAKE, 16, None)
+
+    assert bwd(top) == L.DGX_ENOMEM
+    for n in (top + 1, (1 << 31) - 511, (1 << 31) - 1):
+        assert bwd(n) == L.DGX_EINVAL, n
+        assert b"above" in lib.dgx_last_error()
+        assert lib.dgx_embed_bwd_workspace_size(n, 16, 10) == 0
+
+
 def test_workspace_sizes(lib):
     assert lib.dgx_linear_nll_workspace_size(0, 10, 8, 0) == 0
     assert lib.dgx_linear_distill_workspace_size(4, 10, 8, 300, 1) == 0

@@ -49,7 +49,8 @@ __device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepco
 // One warp per row: q = softmax(teacher / T) over the entries whose id lies in
 // [0, V), and the entries in ascending order of (id, position), absent ones
 // last (id kNoId, q 0). A teacher logit of -inf has q = 0; a row whose entries
-// are all absent or -inf has live = 0. The rank of an entry is the number of
+// are all absent or -inf has live = 0 (a NaN entry is neither: its row has a
+// target, and NaN results). The rank of an entry is the number of
 // entries before it, counted four ids per shared-memory load. start[row][s] is
 // the first entry whose id is at least kHeadSlot s. KI: entries per lane.
 // Latency of two dependent loads and the ranking: 5 us at 333 rows of 17.
@@ -69,6 +70,7 @@ __global__ void __launch_bounds__(128) head_lists_kernel(const int* __restrict__
   int id[KI];
   float q[KI];
   float mx = -INFINITY;
+  bool some = false;
 #pragma unroll
   for (int i = 0; i < KI; ++i) {
     const int k = lane + 32 * i;
@@ -80,13 +82,14 @@ __global__ void __launch_bounds__(128) head_lists_kernel(const int* __restrict__
       if (v >= 0 && v < V) {
         id[i] = v;
         q[i] = l;
-        mx = fmaxf(mx, l);
+        mx = fmaxf(mx, l);  // drops a NaN
+        some |= l != -INFINITY;
       }
     }
     ids[k] = id[i];
   }
   mx = warp_max(mx);
-  const bool any = mx != -INFINITY;
+  const bool any = __any_sync(0xffffffffu, some);
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < KI; ++i) {

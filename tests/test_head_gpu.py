@@ -276,6 +276,34 @@ def test_teacher_mask_values(dgx):
     p.check_bwd(*p.bwd(dgx, lse))
 
 
+@pytest.mark.parametrize("K", [1, 12, 200])
+def test_nan_teacher_rows_are_not_empty_rows(dgx, K):
+    """A NaN teacher logit gives its row a NaN loss and gradient, whether it is the row's only entry, one of several
+    or beside entries of -inf; the other rows keep their bits. A NaN at an absent entry does not count."""
+    p = Problem(70, 300, 64, K=K, seed=30)
+    loss0, lse0 = p.fwd(dgx)
+    dH0, _, _ = p.bwd(dgx, lse0)
+    hit = [5, 33, 66]
+    p.teacher[5] = float("nan")
+    p.teacher[33, -1] = float("nan")
+    p.teacher[66] = float("-inf")
+    p.teacher[66, 0] = float("nan")
+    p.idx[40, 0] = -1
+    loss1 = p.fwd(dgx)[0]
+    p.teacher[40, 0] = float("nan")
+    loss, lse = p.fwd(dgx)
+    dH, dW, _ = p.bwd(dgx, lse)
+    keep = torch.ones(70, dtype=torch.bool, device="cuda")
+    keep[hit] = False
+    assert torch.equal(loss[keep], loss1[keep]) and torch.isfinite(loss[keep]).all()
+    keep[40] = False
+    assert torch.equal(loss[keep], loss0[keep]) and torch.equal(lse, lse0) and torch.equal(dH[keep], dH0[keep])
+    assert loss[hit].isnan().all() and dH[hit].isnan().all()
+    named = torch.zeros(300, dtype=torch.bool, device="cuda")
+    named[p.idx[hit].long()] = True
+    assert dW[named].isnan().all() and torch.isfinite(dW[~named]).all()
+
+
 def test_non_finite_rows_stay_in_their_rows(dgx):
     """A NaN hidden row gives a NaN loss and dH in that row alone; a row without
     a target keeps loss 0 and dH 0 whatever it holds."""

@@ -22,8 +22,11 @@ vocabulary run on the operators made for it: the embedding with a scale and its
 gradient summed in token order (dgx_embed_fwd / dgx_embed_bwd), and the output
 layer, softmax and loss in one operator that keeps no logits
 (dgx_linear_nll_fwd / _bwd). ``teacher_k`` > 0 adds distillation from a
-teacher's largest logits (dgx_linear_distill_fwd / _bwd; ``set_teacher``): the
-loss becomes (1 - a) nll + a distillation with a = ``teacher_weight``.
+teacher's largest logits (dgx_linear_distill_fwd / _bwd; ``set_teacher``, before
+which no position has a teacher and that part is 0): the loss, returned and in
+``loss``, becomes (1 - a) nll + a distillation with a = ``teacher_weight``; its
+parts are in ``nll_loss`` and ``distill_loss``. A part of weight 0 is reported
+but enters neither the loss nor its gradient.
 """
 from __future__ import annotations
 
@@ -160,8 +163,12 @@ class GPT:
         if K:
             self.teacher_idx = torch.full((R, K), -1, device=dev, dtype=torch.int32)
             self.teacher_logits = torch.zeros(R, K, device=dev, dtype=torch.float32)
-            self.distill_loss = torch.zeros(1, device=dev, dtype=torch.float32)
+            self.parts = torch.zeros(2, device=dev, dtype=torch.float32)
+            self.nll_loss, self.distill_loss = self.parts[:1], self.parts[1:]
+            self.shares = torch.tensor([1.0 - c.teacher_weight, c.teacher_weight], device=dev)
             need += [linear_distill_workspace_size(R, V, d, K, b) for b in (False, True)]
+        else:
+            self.nll_loss = self.loss
         self.vocab_ws = torch.empty(max(need), device=dev, dtype=torch.uint8)
 
     # ------------------------------------------------------------ setup
@@ -225,15 +232,20 @@ class GPT:
         c, R, V, ws = self.cfg, self.R, self.cfg.vocab, self.vocab_ws
         W, b = self.w16["Wout"][:V], self.p["bout"][:V]
         out = dict(bias=b, dH=self.dh, dW=self.g["Wout"][:V], db=self.g["bout"][:V], workspace=ws)
-        share = 1.0 - c.teacher_weight if c.teacher_k else 1.0
-        linear_nll_fwd(hf, W, self.tgt, bias=b, loss=self.row_loss, lse=self.row_lse, mean=self.loss, workspace=ws)
-        linear_nll_bwd(hf, W, self.tgt, self.row_lse, scale=share / R, **out)
+        a = c.teacher_weight if c.teacher_k else 0.0
+        linear_nll_fwd(hf, W, self.tgt, bias=b, loss=self.row_loss, lse=self.row_lse, mean=self.nll_loss, workspace=ws)
+        if a != 1.0:
+            linear_nll_bwd(hf, W, self.tgt, self.row_lse, scale=(1.0 - a) / R, **out)
         if c.teacher_k:
             t = (self.teacher_idx, self.teacher_logits)
             linear_distill_fwd(hf, W, *t, bias=b, temperature=c.temperature, loss=self.row_loss, lse=self.row_lse,
                                mean=self.distill_loss, workspace=ws)
-            linear_distill_bwd(hf, W, *t, self.row_lse, temperature=c.temperature, scale=c.teacher_weight / R,
-                               accumulate=True, accumulate_dH=True, **out)
+            if a != 0.0:
+                linear_distill_bwd(hf, W, *t, self.row_lse, temperature=c.temperature, scale=a / R, accumulate=a != 1.0,
+                                   accumulate_dH=a != 1.0, **out)
+            # loss = shares . parts, over the parts that count
+            k0, k1 = int(a == 1.0), 1 + int(a != 0.0)
+            gemm(self.parts[None, k0:k1], self.shares[k0:k1, None], out=self.loss[:, None], f32_mode=L.DGX_F32_FFMA)
 
     # ------------------------------------------------------------ step
     def forward_backward(self):

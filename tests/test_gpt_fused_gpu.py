@@ -137,6 +137,47 @@ def test_distillation_pulls_the_student_to_the_teacher(dgx):
     assert losses[-1][0] < 0.5 * losses[0][0]
 
 
+@pytest.mark.parametrize("weight", [0.0, 0.25, 0.75, 1.0])
+def test_the_loss_returned_is_the_one_minimised(dgx, weight):
+    """(1 - a) nll + a distillation, against its parts and against the gradient of the output bias, which the two
+    losses and nothing else in the step depend on linearly."""
+    m = make(True, teacher_k=6, teacher_weight=weight, temperature=2.0)
+    batch(m)
+    n = m.cfg.batch * m.cfg.seq_len
+    g = torch.Generator().manual_seed(5)
+    m.set_teacher(torch.randint(0, 20, (n, 6), generator=g).to(torch.int32), 4 * torch.randn(n, 6, generator=g))
+    got = m.forward_backward()
+    nll, distill, loss = m.nll_loss.item(), m.distill_loss.item(), got.item()
+    assert got is m.loss and nll > 1.0 and distill > 1.0
+    # two products and a sum in fp32
+    assert abs(loss - ((1 - weight) * nll + weight * distill)) <= 3 * 2.0 ** -24 * max(nll, distill)
+    # A step h along a direction of signs: the cubic term of a log-sum-exp along it is at most h^2 / 6 (its third
+    # central moment over values of +-1 is below 1, T^2 / T^3 < 1); either end's loss is a mean of rows that are
+    # 1e-5 off at most and the gradient sums n rows of fp32 probabilities (1e-5 of at most 2 per row).
+    h, grad = 2.0 ** -5, m.g["bout"][:65].clone()
+    sign = torch.where(grad < 0, -1.0, 1.0)
+    ends = []
+    for step in (h, -2 * h):
+        m.p["bout"][:65] += step * sign
+        ends.append(m.forward_backward().item())
+    slope, along = (ends[0] - ends[1]) / (2 * h), float((grad * sign).sum())
+    assert along > 0.1
+    assert abs(slope - along) <= h * h / 6 + 1e-5 / h + 2e-5
+
+
+def test_a_loss_of_weight_zero_does_not_touch_the_gradient(dgx):
+    """A masked target makes the hard loss infinite; with all weight on the teacher the step stays finite."""
+    m = make(True, teacher_k=3, teacher_weight=1.0)
+    batch(m)
+    n = m.cfg.batch * m.cfg.seq_len
+    m.p["bout"][int(m.tgt[0])] = float("-inf")
+    ids = (m.tgt[0].cpu() + 1 + torch.arange(3)).remainder(65).to(torch.int32).repeat(n, 1)
+    m.set_teacher(ids, torch.zeros(n, 3))
+    loss = m.forward_backward().item()
+    assert m.nll_loss.item() == float("inf") and loss == m.distill_loss.item() and 0 < loss < float("inf")
+    assert all(torch.isfinite(v).all() for v in m.g.values())
+
+
 def test_options_need_the_fused_step(dgx):
     for kw in (dict(teacher_k=4), dict(embed_scale=2.0)):
         with pytest.raises(AssertionError):

@@ -252,9 +252,10 @@ def _ws(workspace: Optional[torch.Tensor]):
     return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
 
 
-def _head_check(H, W, bias, rows32, rowsf, mean=None):
-    """Shapes and types shared by the vocabulary-head wrappers; returns (R, V,
-    d) and the row pitches of H and W. Each attribute of a tensor is asked for
+def _head_check(H, W, bias, ids, K, rowsf, mean=None):
+    """Shapes and types shared by the vocabulary-head wrappers (ids: K per row,
+    rowsf: one fp32 element per row); returns (R, V, d) and the row pitches of
+    H and W. Each attribute of a tensor is asked for
     once: for a few rows these checks weigh as much as the kernels."""
     dev = H.get_device()
     assert dev >= 0 and H.dtype is torch.bfloat16 and H.dim() == 2, "H: [R, d] bf16 CUDA rows"
@@ -264,14 +265,23 @@ def _head_check(H, W, bias, rows32, rowsf, mean=None):
     assert (sh == 1 or d == 1) and (sw == 1 or d == 1), "the columns of H and W must be contiguous"
     if bias is not None:
         assert bias.get_device() == dev and bias.dtype is torch.float32 and bias.is_contiguous() and bias.numel() == V
-    assert rows32.get_device() == dev and rows32.dtype is torch.int32 and rows32.is_contiguous() and rows32.shape[0] == R
+    assert ids.get_device() == dev and ids.dtype is torch.int32 and ids.is_contiguous() and ids.numel() == R * K, \
+        "target or idx: int32, one row of ids per row of H"
     for t in rowsf:
         if t is not None:
-            assert t.get_device() == dev and t.dtype is torch.float32 and t.is_contiguous() and t.shape[0] == R
+            assert t.get_device() == dev and t.dtype is torch.float32 and t.is_contiguous() and t.numel() == R, \
+                "loss, lse and dloss: one fp32 element per row of H"
     if mean is not None:
         assert mean.get_device() == dev and mean.dtype is torch.float32 and mean.numel() == 1, "mean: one fp32 element"
     # torch reports any stride for a single row
     return R, V, d, ldh if R > 1 else (d + 7) // 8 * 8, ldw if V > 1 else (d + 7) // 8 * 8
+
+
+def _teacher_check(idx, teacher) -> int:
+    assert idx.dim() == 2 and teacher.shape == idx.shape, "idx and teacher: [R, K]"
+    assert teacher.get_device() == idx.get_device() and teacher.dtype is torch.float32 and teacher.is_contiguous(), \
+        "teacher: contiguous fp32 logits on idx's device"
+    return idx.shape[1]
 
 
 def _grad_out(out, want: bool, rows: int, d: int, device, dev: int):
@@ -296,8 +306,8 @@ def linear_nll_fwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, *, bi
     int32 (outside [0, V): no target, loss 0). Returns (loss [R], lse [R]), the
     row log-sum-exp being what linear_nll_bwd needs; `mean` (one fp32 element)
     receives sum(loss) / R."""
-    R, V, d, ldh, ldw = _head_check(H, W, bias, target, (loss, lse), mean)
-    assert target.dim() == 1
+    R, V, d, ldh, ldw = _head_check(H, W, bias, target, 1, (loss, lse), mean)
+    assert target.dim() == 1, "target: [R]"
     if loss is None:
         loss = torch.empty(R, device=H.device, dtype=torch.float32)
     if lse is None:
@@ -317,7 +327,8 @@ def linear_nll_bwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, lse: 
     (dH [R, d], dW [V, d], db [V] fp32); those not in `need` (and db without a
     bias) are None. dH and dW are new bf16 tensors unless given (bf16 or fp32);
     accumulate adds to the given fp32 dW and db, accumulate_dH to the fp32 dH."""
-    R, V, d, ldh, ldw = _head_check(H, W, bias, target, (lse, dloss))
+    R, V, d, ldh, ldw = _head_check(H, W, bias, target, 1, (lse, dloss))
+    assert target.dim() == 1, "target: [R]"
     dH, dW, db, grads = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH)
     ws, wsb = _ws(workspace)
     L.call("dgx_linear_nll_bwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), target.data_ptr(),
@@ -352,15 +363,15 @@ def linear_distill_fwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teac
     against a teacher's K largest logits per row: idx [R, K] int32 vocabulary
     ids (outside [0, V): absent), teacher [R, K] fp32. Returns (loss [R],
     lse [R]) with lse the log-sum-exp of the student's logits / T."""
-    R, V, d, ldh, ldw = _head_check(H, W, bias, idx, (teacher, loss, lse), mean)
-    assert idx.dim() == 2 and teacher.shape == idx.shape
+    K = _teacher_check(idx, teacher)
+    R, V, d, ldh, ldw = _head_check(H, W, bias, idx, K, (loss, lse), mean)
     if loss is None:
         loss = torch.empty(R, device=H.device, dtype=torch.float32)
     if lse is None:
         lse = torch.empty(R, device=H.device, dtype=torch.float32)
     ws, wsb = _ws(workspace)
     L.call("dgx_linear_distill_fwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), idx.data_ptr(),
-           teacher.data_ptr(), idx.shape[1], float(temperature), R, V, d, loss.data_ptr(), lse.data_ptr(), _ptr(mean),
+           teacher.data_ptr(), K, float(temperature), R, V, d, loss.data_ptr(), lse.data_ptr(), _ptr(mean),
            ws, wsb, _stream(H))
     return loss, lse
 
@@ -371,12 +382,12 @@ def linear_distill_bwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teac
                        dW: Optional[torch.Tensor] = None, db: Optional[torch.Tensor] = None,
                        need=("dH", "dW", "db"), accumulate: bool = False, accumulate_dH: bool = False, workspace: Optional[torch.Tensor] = None):
     """Gradients of sum_r scale * dloss[r] * loss[r]; arguments and results as linear_nll_bwd."""
-    R, V, d, ldh, ldw = _head_check(H, W, bias, idx, (teacher, lse, dloss))
-    assert idx.dim() == 2 and teacher.shape == idx.shape
+    K = _teacher_check(idx, teacher)
+    R, V, d, ldh, ldw = _head_check(H, W, bias, idx, K, (lse, dloss))
     dH, dW, db, grads = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH)
     ws, wsb = _ws(workspace)
     L.call("dgx_linear_distill_bwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), idx.data_ptr(),
-           teacher.data_ptr(), idx.shape[1], float(temperature), lse.data_ptr(), _ptr(dloss), float(scale), R, V, d,
+           teacher.data_ptr(), K, float(temperature), lse.data_ptr(), _ptr(dloss), float(scale), R, V, d,
            *grads, int(accumulate) + 2 * int(accumulate_dH), ws, wsb,
            _stream(H))
     return dH, dW, db

@@ -500,3 +500,25 @@ def test_mean_must_be_one_float_on_the_device(dgx):
             dgx.linear_nll_fwd(H, W, t, mean=bad)
         with pytest.raises(AssertionError, match="mean"):
             dgx.linear_distill_fwd(H, W, t[:, None], torch.zeros(8, 1, device="cuda"), mean=bad)
+
+
+def test_row_arguments_hold_one_element_per_row(dgx):
+    """Tensors whose first extent alone is the number of rows would be read as their leading elements."""
+    H = torch.zeros(8, 64, device="cuda", dtype=torch.bfloat16)
+    W = torch.zeros(100, 64, device="cuda", dtype=torch.bfloat16)
+    t = torch.zeros(8, device="cuda", dtype=torch.int32)
+    row, rows = torch.zeros(8, device="cuda"), torch.zeros(8, 3, device="cuda")
+    i3 = torch.zeros(8, 3, device="cuda", dtype=torch.int32)
+    for wrong in (lambda: dgx.linear_nll_fwd(H, W, i3), lambda: dgx.linear_nll_bwd(H, W, i3, row),
+                  lambda: dgx.linear_nll_fwd(H, W, t, loss=rows), lambda: dgx.linear_nll_fwd(H, W, t, lse=rows),
+                  lambda: dgx.linear_nll_bwd(H, W, t, rows), lambda: dgx.linear_nll_bwd(H, W, t, row, dloss=rows),
+                  lambda: dgx.linear_distill_fwd(H, W, i3, rows, lse=rows),
+                  lambda: dgx.linear_distill_bwd(H, W, i3, rows, rows),
+                  lambda: dgx.linear_distill_bwd(H, W, i3, rows, row, dloss=rows),
+                  lambda: dgx.linear_distill_fwd(H, W, i3, rows.double()),
+                  lambda: dgx.linear_distill_fwd(H, W, i3, torch.zeros(3, 8, device="cuda").T),
+                  lambda: dgx.linear_distill_fwd(H, W, torch.zeros(7, 3, device="cuda", dtype=torch.int32), rows[:7])):
+        with pytest.raises(AssertionError):
+            wrong()
+    dgx.linear_distill_bwd(H, W, i3, rows, dgx.linear_distill_fwd(H, W, i3, rows)[1], dloss=row)
+    dgx.sync_check()

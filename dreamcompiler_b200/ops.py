@@ -248,8 +248,12 @@ def linear_distill_workspace_size(R: int, V: int, d: int, K: int, backward: bool
 _ROW_DT = {torch.float32: L.DGX_F32, torch.bfloat16: L.DGX_BF16}
 
 
-def _ws(workspace: Optional[torch.Tensor]):
-    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+def _ws(workspace: Optional[torch.Tensor], dev: int):
+    """A workspace's pointer and bytes: whole memory of the operands' device, since kernels write all over it."""
+    if workspace is None:
+        return None, 0
+    assert workspace.get_device() == dev and workspace.is_contiguous(), "workspace: contiguous, on the operands' device"
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def _head_check(H, W, bias, ids, K, rowsf, mean=None):
@@ -312,7 +316,7 @@ def linear_nll_fwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, *, bi
         loss = torch.empty(R, device=H.device, dtype=torch.float32)
     if lse is None:
         lse = torch.empty(R, device=H.device, dtype=torch.float32)
-    ws, wsb = _ws(workspace)
+    ws, wsb = _ws(workspace, H.get_device())
     L.call("dgx_linear_nll_fwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), target.data_ptr(), R, V,
            d, loss.data_ptr(), lse.data_ptr(), _ptr(mean), ws, wsb, _stream(H))
     return loss, lse
@@ -330,7 +334,7 @@ def linear_nll_bwd(H: torch.Tensor, W: torch.Tensor, target: torch.Tensor, lse: 
     R, V, d, ldh, ldw = _head_check(H, W, bias, target, 1, (lse, dloss))
     assert target.dim() == 1, "target: [R]"
     dH, dW, db, grads = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH)
-    ws, wsb = _ws(workspace)
+    ws, wsb = _ws(workspace, H.get_device())
     L.call("dgx_linear_nll_bwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), target.data_ptr(),
            lse.data_ptr(), _ptr(dloss), float(scale), R, V, d, *grads,
            int(accumulate) + 2 * int(accumulate_dH), ws, wsb, _stream(H))
@@ -369,7 +373,7 @@ def linear_distill_fwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teac
         loss = torch.empty(R, device=H.device, dtype=torch.float32)
     if lse is None:
         lse = torch.empty(R, device=H.device, dtype=torch.float32)
-    ws, wsb = _ws(workspace)
+    ws, wsb = _ws(workspace, H.get_device())
     L.call("dgx_linear_distill_fwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), idx.data_ptr(),
            teacher.data_ptr(), K, float(temperature), R, V, d, loss.data_ptr(), lse.data_ptr(), _ptr(mean),
            ws, wsb, _stream(H))
@@ -385,7 +389,7 @@ def linear_distill_bwd(H: torch.Tensor, W: torch.Tensor, idx: torch.Tensor, teac
     K = _teacher_check(idx, teacher)
     R, V, d, ldh, ldw = _head_check(H, W, bias, idx, K, (lse, dloss))
     dH, dW, db, grads = _head_grads(H, bias, R, V, d, dH, dW, db, need, accumulate, accumulate_dH)
-    ws, wsb = _ws(workspace)
+    ws, wsb = _ws(workspace, H.get_device())
     L.call("dgx_linear_distill_bwd", H.data_ptr(), ldh, W.data_ptr(), ldw, _ptr(bias), idx.data_ptr(),
            teacher.data_ptr(), K, float(temperature), lse.data_ptr(), _ptr(dloss), float(scale), R, V, d,
            *grads, int(accumulate) + 2 * int(accumulate_dH), ws, wsb,
@@ -438,7 +442,7 @@ def embed_bwd(tok: torch.Tensor, dx: torch.Tensor, V: int, *, scale: float = 1.0
         out = torch.empty(V, d, device=dx.device, dtype=out_dtype)
     wt, (lddw, so) = _ROW_DT.get(out.dtype), out.stride()
     assert out.get_device() == dev and out.shape == (V, d) and (so == 1 or d == 1) and wt is not None
-    ws, wsb = _ws(workspace)
+    ws, wsb = _ws(workspace, dev)
     L.call("dgx_embed_bwd", tok.data_ptr(), dx.data_ptr(), gt, lddx if n > 1 else d, float(scale), out.data_ptr(), wt,
            lddw if V > 1 else d, n, d, V, int(accumulate), ws, wsb, _stream(dx))
     return out

@@ -196,3 +196,11 @@ def test_refusals(dgx):
                   lambda: dgx.embed_bwd(tok, dx, 10, out=torch.zeros(9, 16, device="cuda"))):
         with pytest.raises(AssertionError):
             wrong()
+
+
+def test_workspace_must_be_on_the_device(dgx):
+    tok = torch.zeros(4, device="cuda", dtype=torch.int32)
+    dx = torch.zeros(4, 16, device="cuda")
+    for bad in (torch.empty(1 << 20), torch.empty(1, device="cuda").expand(1 << 20)):
+        with pytest.raises(AssertionError, match="workspace"):
+            dgx.embed_bwd(tok, dx, 10, workspace=bad)

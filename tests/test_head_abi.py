@@ -133,3 +133,16 @@ def test_faults_can_be_injected(lib):
             assert b"injected fault" in lib.dgx_last_error()
     finally:
         lib.dgx_fault_inject(0, 0)
+
+
+def test_workspace_tensors_are_whole_and_on_the_device():
+    """A host tensor, or an expanded one whose bytes are not there, would be written by the kernels."""
+    import torch
+    from dreamcompiler_b200.ops import _ws
+    assert _ws(None, 0) == (None, 0)
+    host = torch.empty(64, dtype=torch.uint8)
+    assert _ws(host, host.get_device()) == (host.data_ptr(), 64)
+    with pytest.raises(AssertionError, match="workspace"):
+        _ws(host, 0)
+    with pytest.raises(AssertionError, match="workspace"):
+        _ws(torch.empty(1).expand(1 << 20), -1)

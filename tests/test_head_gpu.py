@@ -522,3 +522,16 @@ def test_row_arguments_hold_one_element_per_row(dgx):
             wrong()
     dgx.linear_distill_bwd(H, W, i3, rows, dgx.linear_distill_fwd(H, W, i3, rows)[1], dloss=row)
     dgx.sync_check()
+
+
+def test_workspace_must_be_on_the_device(dgx):
+    H = torch.zeros(8, 64, device="cuda", dtype=torch.bfloat16)
+    t, row = torch.zeros(8, device="cuda", dtype=torch.int32), torch.zeros(8, device="cuda")
+    i1, q1 = t[:, None], row[:, None]
+    for bad in (torch.empty(1 << 20), torch.empty(1, device="cuda").expand(1 << 20)):
+        for call in (lambda: dgx.linear_nll_fwd(H, H, t, workspace=bad),
+                     lambda: dgx.linear_nll_bwd(H, H, t, row, workspace=bad),
+                     lambda: dgx.linear_distill_fwd(H, H, i1, q1, workspace=bad),
+                     lambda: dgx.linear_distill_bwd(H, H, i1, q1, row, workspace=bad)):
+            with pytest.raises(AssertionError, match="workspace"):
+                call()

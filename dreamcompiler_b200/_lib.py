@@ -106,18 +106,19 @@ _fns = {}  # name -> bound entry point, filled by load()
 
 def load(path: str = LIB_PATH) -> C.CDLL:
     """Load libdgx.so (built by dreamcompiler_b200.build) and bind signatures."""
-    global _lib
+    global _lib, _fns
     if _lib is not None:
         return _lib
     if not os.path.exists(path):
         raise ImportError(f"libdgx.so not built at {path}; run python -m dreamcompiler_b200.build")
     lib = C.CDLL(path, mode=C.RTLD_GLOBAL)
+    fns = {}
     for name, (res, args) in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
-        _fns[name] = fn
-    _lib = lib
+        fns[name] = fn
+    _fns, _lib = fns, lib  # all of them or none: another thread may be in call(), and a symbol may be missing
     return lib
 
 

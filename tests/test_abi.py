@@ -115,3 +115,40 @@ def test_reference_runtime_with_b200_backend_loads():
               "dream_tp_matmul_column", "dream_set_precision", "dream_b200_count"):
         assert hasattr(rt, n)
     assert rt.dream_b200_count(0) == 0 and rt.dream_b200_count(99) == -1
+
+
+class StubLibrary:
+    """Hands out entry points that return `status`, up to a symbol it lacks; `seen` notes the bound names visible to
+    other threads at each lookup."""
+
+    def __init__(self, L, missing=None):
+        self._L, self._missing, self.seen = L, missing, []
+
+    def __getattr__(self, name):
+        if name == self._missing:
+            raise AttributeError(name)
+        self.seen.append(len(self._L._fns))
+        fn = lambda *args: 0  # noqa: E731
+        setattr(self, name, fn)
+        return fn
+
+
+@pytest.mark.parametrize("missing", [None, "dgx_embed_fwd"])
+def test_entry_points_are_bound_all_or_none(monkeypatch, missing):
+    """A call from another thread during the first load sees no half-filled table, and a library that lacks a symbol
+    leaves nothing behind that later calls would run on."""
+    from dreamcompiler_b200 import _lib as L
+    stub = StubLibrary(L, missing)
+    monkeypatch.setattr(L, "_lib", None)
+    monkeypatch.setattr(L, "_fns", {})
+    monkeypatch.setattr(L.C, "CDLL", lambda *a, **k: stub)
+    if missing:
+        with pytest.raises(AttributeError):
+            L.load()
+        assert not L._fns and L._lib is None
+        with pytest.raises(AttributeError):
+            L.call("dgx_version")
+    else:
+        L.call("dgx_init", 0)
+        assert set(L._fns) == set(L.SIGNATURES) and L._lib is stub
+    assert stub.seen and not any(stub.seen)

@@ -13,6 +13,7 @@
 // scatter-add of repeated token ids).
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "common.h"
@@ -694,14 +695,15 @@ dgx_status dgx_colsum(const void* dy, int dy_type, float* db, int R, int N, int 
   if (!dy || !db) return set_error(DGX_EINVAL, "dgx_colsum: null pointer");
   cudaStream_t s = (cudaStream_t)stream;
   constexpr int kMaxSlices = 128;
-  float* part = (float*)library_scratch((size_t)kMaxSlices * N * sizeof(float), s);
-  if (!part) return set_error(DGX_ENOMEM, "dgx_colsum: scratch");
   const int esz = dy_type == DGX_F32 ? 4 : 2, vec = 16 / esz;
+  const bool vectors = N % vec == 0 && ((uintptr_t)dy & 15) == 0;
+  const int cblocks = vectors ? (N / vec + 31) / 32 : 0;
   int slices = CS_SLICES;
-  if (N % vec == 0 && ((uintptr_t)dy & 15) == 0) {
-    const int cblocks = (N / vec + 31) / 32;
-    slices = (2 * num_sms() + cblocks - 1) / cblocks;
-    slices = slices < 1 ? 1 : (slices > kMaxSlices ? kMaxSlices : slices);
+  if (vectors) slices = std::max(1, std::min((2 * num_sms() + cblocks - 1) / cblocks, kMaxSlices));
+  // as many rows of partial sums as are used: a wide N has few slices
+  float* part = (float*)library_scratch((size_t)slices * N * sizeof(float), s);
+  if (!part) return set_error(DGX_ENOMEM, "dgx_colsum: scratch");
+  if (vectors) {
     dim3 grid(cblocks, slices);
     if (dy_type == DGX_F32)
       colsum_partial_vec_kernel<float><<<grid, 256, 0, s>>>((const float*)dy, part, R, N, slices);

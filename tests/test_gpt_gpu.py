@@ -228,3 +228,31 @@ def test_head_layout_kernels(dgx, src_type):
     assert torch.equal(heads, ref)
     assert torch.equal(back[:, col0:col0 + H * D], rows[:, col0:col0 + H * D].bfloat16())
     assert not back[:, :col0].any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_colsum_scratch_follows_its_slices(dgx, dtype):
+    """Few rows of very many columns (the position table's gradient: batch rows of seq_len * d_model columns) are one
+    row slice: 32 MB of partial sums at 2^23 columns, where 128 slices would be 4 GB. In a process of its own, as the
+    library keeps its scratch."""
+    import subprocess
+    import sys
+    code = f"""
+import torch, dreamcompiler_b200 as dgx
+from dreamcompiler_b200 import _lib as L
+dgx.init(0)
+N = 1 << 23
+x = torch.randn(3, N, device="cuda").to(torch.{'bfloat16' if dtype == 'bf16' else 'float32'})
+o = torch.empty(N, device="cuda")
+torch.cuda.synchronize()
+free = torch.cuda.mem_get_info()[0]
+L.call("dgx_colsum", x.data_ptr(), L.DGX_{'BF16' if dtype == 'bf16' else 'F32'}, o.data_ptr(), 3, N, 0,
+       torch.cuda.current_stream().cuda_stream)
+dgx.sync_check()
+took = free - torch.cuda.mem_get_info()[0]
+want = x.double().sum(0)
+assert bool(((o.double() - want).abs() <= 2.0 ** -22 * x.double().abs().sum(0)).all())
+assert took <= 256 << 20, took
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

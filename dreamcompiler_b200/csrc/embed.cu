@@ -173,10 +173,8 @@ struct SortArgs {
 };
 
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortArgs a) {
-  // in this order: the zeroing kernel does not wait for anything itself, so it
-  // may start only when all that came before this call is done
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ int hist[];              // [kSortWarps][bins]
   cg::cluster_group cluster = cg::this_cluster();
   const int ncta = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
@@ -301,88 +299,6 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortArgs a) {
   }
 }
 
-// ---------------------------------------------------------------- rows without a token
-// Zeroes the rows of dW whose token does not occur, on the SMs that the sort's
-// CTAs leave free. The table is cut into groups of 32 rows dealt out in turn to
-// 512 CTAs, all resident (148 took 121 us for 537 MB beside the sort, 512 take
-// 90); a CTA finds the tokens of its groups by reading all ids (4
-// bytes per id and CTA, from L2), so it waits for nothing. The rows go out as
-// bulk copies of a zeroed piece of shared memory, one lane per row. Launched
-// as the sort's dependent; block 0 ends after the sort, so that a kernel that
-// waits for this one waits for both.
-constexpr int kZeroThreads = 512, kZeroCap = 2048;  // groups marked at a time
-constexpr int kZeroBytes = 8192;
-
-struct ZeroArgs {
-  const int* tok;
-  int n, V;
-  char* dW;            // rows of row_bytes, pitch bytes apart
-  size_t pitch;
-  int row_bytes, vec;  // vec: whole 16-byte units
-};
-
-__global__ void __launch_bounds__(kZeroThreads) embed_zero_kernel(ZeroArgs a) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __shared__ unsigned bits[kZeroCap];
-  __shared__ __align__(128) uint4 zeros[kZeroBytes / 16];
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  const int G = gridDim.x, lg = 31 - __clz(G);  // a power of two
-  const int groups = (int)(((long long)a.V + 31) / 32);
-  const int mine = (groups - (int)blockIdx.x + G - 1) >> lg;  // groups of this CTA
-  // The ids were complete before the sort let this grid start. It has not
-  // waited for their writer itself, so a line of them that an earlier grid left
-  // in this SM's L1 is dropped here (reading past L1 instead: 64 -> 71 us a
-  // forward and backward of 16381 tokens on 50257 x 1024).
-  if (tid == 0) __threadfence();
-  if (a.vec) {
-    for (int i = tid; i < kZeroBytes / 16; i += kZeroThreads) zeros[i] = make_uint4(0, 0, 0, 0);
-    fence_proxy_async_smem();
-  }
-  for (int g0 = 0; g0 < mine; g0 += kZeroCap) {
-    const int count = min(kZeroCap, mine - g0);
-    __syncthreads();
-    for (int i = tid; i < count; i += kZeroThreads) bits[i] = 0;
-    __syncthreads();
-    auto mark = [&](int t) {
-      const unsigned k = ((unsigned)t >> (5 + lg)) - g0;
-      if ((((unsigned)t >> 5) & (G - 1)) == blockIdx.x && (unsigned)t < (unsigned)a.V && k < (unsigned)count)
-        atomicOr(&bits[k], 1u << (t & 31));
-    };
-    const int n4 = ((uintptr_t)a.tok & 15) ? 0 : a.n >> 2;  // ids four at a time where the array allows
-#pragma unroll 4
-    for (int i = tid; i < n4; i += kZeroThreads) {
-      const int4 t = reinterpret_cast<const int4*>(a.tok)[i];
-      mark(t.x);
-      mark(t.y);
-      mark(t.z);
-      mark(t.w);
-    }
-    for (int i = n4 * 4 + tid; i < a.n; i += kZeroThreads) mark(a.tok[i]);
-    __syncthreads();
-    if (a.vec) {
-      for (int k = w; k < count; k += kZeroThreads / 32) {
-        const long long t = ((long long)(g0 + k) * G + blockIdx.x) * 32 + lane;
-        if (t >= a.V || bits[k] >> lane & 1) continue;
-        char* row = a.dW + (size_t)t * a.pitch;
-        for (int j = 0; j < a.row_bytes; j += kZeroBytes)
-          bulk_store(row + j, zeros, (uint32_t)min(kZeroBytes, a.row_bytes - j));
-      }
-    } else {  // elements are 2 or 4 bytes
-      for (int i = w; i < count * 32; i += kZeroThreads / 32) {
-        const long long t = ((long long)(g0 + (i >> 5)) * G + blockIdx.x) * 32 + (i & 31);
-        if (t >= a.V || bits[i >> 5] >> (i & 31) & 1) continue;
-        char* row = a.dW + (size_t)t * a.pitch;
-        for (int j = lane * 2; j < a.row_bytes; j += 64) *reinterpret_cast<uint16_t*>(row + j) = 0;
-      }
-    }
-  }
-  if (a.vec) {
-    bulk_commit();
-    bulk_wait0();
-  }
-  if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 // ---------------------------------------------------------------- sums
 // The sorted positions are cut evenly, whatever the tokens: a block owns 128
 // positions and 256 columns, each of its 8 warps 16 positions, so no token's
@@ -404,6 +320,7 @@ struct SumArgs {
   int n, d, V, slabs, blocks;
   int lddx, lddw, accumulate;
   float scale;
+  int zero_blocks, bulk;  // blocks that zero rows; rows of dW are whole aligned 16-byte units
 };
 
 template <typename TW, bool VEC>
@@ -425,7 +342,7 @@ __device__ __forceinline__ void finish_row(const SumArgs& a, TW* dW, int t, int 
 }
 
 struct SumShared {
-  float head[8][kSlab];  // element k of lane l at [l + 32 k]
+  float head[8][kSlab];  // element k of lane l at [l + 32 k] (a block that zeroes rows: the zeros)
   int through[8];                        // the warp's positions are one token that comes in and goes on
   int last_token[2], last_block[2], last_parts[2];  // token whose parts are complete (or -1), its blocks
 };
@@ -477,12 +394,67 @@ __device__ __forceinline__ void put_part(const SumArgs& a, SumShared& sh, int bl
   }
 }
 
+// ---------------------------------------------------------------- rows without a token
+// Blocks of the summing launch zero the rows of dW whose token does not occur,
+// kZeroRows rows each: a lane looks its row up in the sorted tokens (all rows
+// at once, so the search's dependent loads cost a few us in all) and sends it
+// out as bulk copies of a zeroed piece of shared memory. These blocks come
+// first: the sums' latency hides behind their writes (gradient of 16381 tokens
+// on 50257 x 1024 fp32 59 us, 62 with them last; 4096 on 32768 x 1024 47
+// against 53; 65536 on 131072 x 2048 bf16 161.5 against 160). 32, 64 or 256 rows
+// a block: 61, 64 and 63 us for the first of these. A launch of its own beside
+// the sort took 52, but would have to read the ids and write dW without having
+// waited for the work before the call.
+constexpr int kZeroRows = 128;
+
+template <typename TW>
+__device__ __forceinline__ void zero_rows(const SumArgs& a, SumShared& sh, TW* dW, unsigned group) {
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (a.bulk) {
+    for (int i = threadIdx.x; i < 8 * kSlab; i += 256) (&sh.head[0][0])[i] = 0.f;
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+  const unsigned t = group * kZeroRows + w * (kZeroRows / 8) + lane;
+  bool absent = lane < kZeroRows / 8 && t < (unsigned)a.V;
+  if (absent) {
+    int lo = 0, hi = a.n;  // first position whose token is t or above
+    while (lo < hi) {
+      const int mid = lo + (hi - lo) / 2;
+      if ((unsigned)a.sorted[mid].x < t)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    absent = lo == a.n || (unsigned)a.sorted[lo].x != t;
+  }
+  if (a.bulk) {
+    const int bytes = a.d * (int)sizeof(TW);
+    char* row = reinterpret_cast<char*>(dW + (size_t)t * a.lddw);
+    if (absent)
+      for (int j = 0; j < bytes; j += (int)sizeof(sh.head))
+        bulk_store(row + j, sh.head, (uint32_t)min((int)sizeof(sh.head), bytes - j));
+    bulk_commit();
+    bulk_wait0();
+  } else {
+    for (unsigned m = __ballot_sync(0xffffffffu, absent); m; m &= m - 1) {
+      TW* row = dW + (size_t)(t - lane + __ffs(m) - 1) * a.lddw;
+      for (int j = lane; j < a.d; j += 32) row[j] = TW(0.f);
+    }
+  }
+}
+
 template <typename TG, typename TW, bool VEC>
 __global__ void __launch_bounds__(256, 4) embed_sum_kernel(const TG* __restrict__ dx, TW* __restrict__ dW, SumArgs a) {
-  __shared__ SumShared sh;
+  __shared__ __align__(16) SumShared sh;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (blockIdx.x < (unsigned)a.zero_blocks) {
+    zero_rows(a, sh, dW, blockIdx.x);
+    return;
+  }
+  const unsigned b = blockIdx.x - a.zero_blocks;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int blk = blockIdx.x / a.slabs, slab = blockIdx.x % a.slabs;
+  const int blk = b / a.slabs, slab = b % a.slabs;
   const int c0 = slab * kSlab, left = a.d - c0;
   if (threadIdx.x < 2) sh.last_token[threadIdx.x] = -1;
   // lanes 0..15: this warp's positions, 16: the one after them, 17: the one before
@@ -590,7 +562,8 @@ __global__ void __launch_bounds__(256, 4) embed_sum_kernel(const TG* __restrict_
 // 256 columns of four rows. One launch instead of three: 100 ids on 5000 x 1024
 // fp32 7 us instead of 12.5. The rows of one token are added by one warp, which
 // bounds kFew (128 equal ids there: 17 us); a table of more than kFewBytes is
-// zeroed faster beside the sort (128 ids on 50257 x 768 fp32: 40 us against 35).
+// zeroed faster by the bulk copies of the sorted form (128 ids on 50257 x 768
+// fp32: 40 us against 36).
 constexpr int kFew = 128;
 constexpr long long kFewBytes = 32ll << 20;
 
@@ -728,14 +701,6 @@ cudaError_t launch_sort(const SortArgs& a, cudaStream_t s) {
   return launch_dependent(embed_sort_kernel, cluster, kSortThreads, kSortWarps * 4 << a.bits, cluster, s, a);
 }
 
-cudaError_t launch_zero(const ZeroArgs& a, cudaStream_t s) {
-  // a power of two of CTAs, a group of rows and 64 KB at least for each
-  const long long units = std::min(((long long)a.V * a.row_bytes + 65535) / 65536, ((long long)a.V + 31) / 32);
-  int ctas = 1;
-  while (ctas < 512 && ctas < units) ctas *= 2;
-  return launch_dependent(embed_zero_kernel, ctas, kZeroThreads, 0, 1, s, a);
-}
-
 template <typename TG, typename TW, bool VEC>
 cudaError_t launch_sum(const int* tok, const void* dx, void* dW, const SumArgs& a, int blocks, bool few, cudaStream_t s) {
   if (few) {
@@ -807,7 +772,8 @@ dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int 
     return cuda_status(cudaMemset2DAsync(dW, lddw * es, 0, d * es, V, s), "dgx_embed_bwd");
   }
   const Layout l = layout(n, d, V);
-  if ((long long)l.blocks * l.slabs > 0x7fffffffll || l.slabs > 65535)
+  const long long zero_blocks = ((long long)V + kZeroRows - 1) / kZeroRows;
+  if ((long long)l.blocks * l.slabs + zero_blocks > 0x7fffffffll || l.slabs > 65535)
     return set_error(DGX_EINVAL, "dgx_embed_bwd: n=%d V=%d d=%d too large", n, V, d);
   char* ws = (char*)workspace;
   if (ws && workspace_bytes < l.bytes)
@@ -841,17 +807,15 @@ dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int 
     so.counters = (int*)(ws + l.counters);
     so.ncounters = l.blocks * l.slabs;
     e = launch_sort(so, s);
-    if (e == cudaSuccess && !accumulate) {
-      ZeroArgs z{tok, n, V, (char*)dW, (size_t)lddw * type_size(dw_type), d * type_size(dw_type), 0};
-      z.vec = (((uintptr_t)dW | z.pitch | (size_t)z.row_bytes) & 15) == 0;
-      e = launch_zero(z, s);
-    }
     if (e != cudaSuccess) return cuda_status(e, "dgx_embed_bwd");
     a.sorted = so.passes & 1 ? so.a : so.b;
     a.counters = so.counters;
     a.parts = (float*)(ws + l.parts);
+    const size_t ts = type_size(dw_type);
+    a.zero_blocks = accumulate ? 0 : (int)zero_blocks;
+    a.bulk = (((uintptr_t)dW | lddw * ts | d * ts) & 15) == 0;
   }
-  const int blocks = l.blocks * l.slabs;
+  const int blocks = l.blocks * l.slabs + a.zero_blocks;
   const bool vec = vec_ok(dx, dx_type, lddx, d) && vec_ok(dW, dw_type, lddw, d);
   const bool g32 = dx_type == DGX_F32, w32 = dw_type == DGX_F32;
   if (g32 && w32)

@@ -8,9 +8,9 @@ namespace dgx {
 
 // Launches `kern` as a programmatic dependent of the kernel before it in the
 // stream: its blocks may be placed, and run up to their griddepcontrol.wait,
-// while that kernel drains. Every kernel launched this way executes the wait
-// before its first access to global memory (or, where its comment says so,
-// before it ends), so the stream's order holds. cluster > 1: thread-block
+// while that kernel drains. Every thread of a kernel launched this way executes
+// the wait before its first access to global memory, so the stream's order
+// holds. cluster > 1: thread-block
 // clusters of that many CTAs.
 template <typename... P, typename... A>
 cudaError_t launch_dependent(void (*kern)(P...), dim3 blocks, int threads, int smem, int cluster, cudaStream_t s,

@@ -1,7 +1,8 @@
 // Vocabulary head: linear layer + softmax + loss with a sparse target, forward
-// and backward, in pieces of the vocabulary. The logits of one piece at a time
-// exist in scratch; what is kept between forward and backward is the row
-// log-sum-exp.
+// and backward, in pieces of the vocabulary. No logit is written to memory: the
+// forward leaves (max, sum) of 64 or 128 columns of a row in scratch, the
+// backward the bf16 gradient G of a piece; what is kept between the two is the
+// row log-sum-exp.
 //
 //   z = (H W^T + b) / T        lse_r = log sum_j exp(z_rj)
 //   hard target t_r:           loss_r = lse_r - z_{r,t}
@@ -52,13 +53,13 @@ __device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepco
 // are all absent or -inf has live = 0 (a NaN entry is neither: its row has a
 // target, and NaN results). The rank of an entry is the number of
 // entries before it, counted four ids per shared-memory load. start[row][s] is
-// the first entry whose id is at least kHeadSlot s. KI: entries per lane.
+// the first entry whose id is at least kHeadSlot (slot0 + s). KI: entries per lane.
 // Latency of two dependent loads and the ranking: 5 us at 333 rows of 17.
 template <int KI>
 __global__ void __launch_bounds__(128) head_lists_kernel(const int* __restrict__ idx, const float* __restrict__ teacher,
                                                          int R, int V, int K, float inv_t, int* __restrict__ sid,
                                                          float* __restrict__ sq, float* __restrict__ live,
-                                                         uint16_t* __restrict__ start, int slots) {
+                                                         uint16_t* __restrict__ start, int slots, int slot0) {
   __shared__ __align__(16) int ids_s[4][KI * 32], sorted_s[4][KI * 32];
   dependents_may_start();
   wait_for_predecessor();
@@ -124,18 +125,63 @@ __global__ void __launch_bounds__(128) head_lists_kernel(const int* __restrict__
     int lo = 0;  // entries below kHeadSlot t: a binary descent over KI * 32 entries
 #pragma unroll
     for (int step = KI * 32; step; step >>= 1)
-      if (lo + step <= KI * 32 && sorted[lo + step - 1] < t * kHeadSlot) lo += step;
+      if (lo + step <= KI * 32 && sorted[lo + step - 1] < (slot0 + t) * kHeadSlot) lo += step;
     start[(size_t)row * slots + t] = (uint16_t)min(lo, K);
   }
 }
 
 // ---------------------------------------------------------------- forward
-// lse and loss from the statistics part[slot][R] (max of the raw logits and
-// sum of exp((z - max) / T) over the slot's columns; without a hard target's
-// column, which nll_row adds). A block owns 32 rows, one
-// per lane; its NW warps walk the slots, eight loads in flight, and their
-// results are joined in warp order. Hard target: sq == null. Latency: 4 us past
-// the logits kernel at 512 rows of 256 slots, 8 us at 333 rows of 786.
+// The statistics of a block's 32 rows over `slots` slots part[slot][R] (max of
+// the raw logits and sum of exp((z - max) / T) over the slot's columns; without
+// a hard target's column, which nll_row adds), one row per lane: the NW warps
+// walk the slots, eight loads in flight, and their results are joined in warp
+// order. Valid in warp 0.
+template <int NW>
+__device__ __forceinline__ void join_slots(const float2* part, int slots, int R, float inv_t,
+                                           float2 (&ms)[NW][32], float& m, float& s, float& base) {
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * 32 + lane;
+  m = -INFINITY;
+  s = 0.f;
+  if (row < R)
+    for (int i = w; i < slots; i += 8 * NW) {
+      float2 p[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        p[u] = i + u * NW < slots ? part[(size_t)(i + u * NW) * R + row] : make_float2(-INFINITY, 0.f);
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) mn = fmaxf(mn, p[u].x);
+      const float b = mn == -INFINITY ? 0.f : mn;
+      s *= expf((m - b) * inv_t);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += p[u].y * expf((p[u].x - b) * inv_t);
+      m = mn;
+    }
+  ms[w][lane] = make_float2(m, s);
+  __syncthreads();
+  if (w) return;
+#pragma unroll
+  for (int i = 1; i < NW; ++i) m = fmaxf(m, ms[i][lane].x);
+  base = m == -INFINITY ? 0.f : m;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) s += ms[i][lane].y * expf((ms[i][lane].x - base) * inv_t);
+}
+
+// One slot out[R] of the statistics in place of `slots` of them: between the
+// pieces of a forward that has several. out may be the first of them.
+__global__ void __launch_bounds__(1024) head_join_kernel(const float2* part, int slots, int R, float inv_t, float2* out) {
+  __shared__ float2 ms[32][32];
+  wait_for_predecessor();
+  float m, s, base;
+  join_slots<32>(part, slots, R, inv_t, ms, m, s, base);
+  const int row = blockIdx.x * 32 + threadIdx.x;
+  if (threadIdx.x < 32 && row < R) out[row] = make_float2(m, s);
+}
+
+// lse and loss of 32 rows per block from the statistics. Hard target: sq ==
+// null. Latency: 4 us past the logits kernel at 512 rows of 256 slots, 8 us at
+// 333 rows of 786.
 template <int NW>
 __global__ void __launch_bounds__(NW * 32) head_finish_kernel(
     const float2* __restrict__ part, int slots, int R, int V, float t, float inv_t, const int* __restrict__ sid,
@@ -146,31 +192,9 @@ __global__ void __launch_bounds__(NW * 32) head_finish_kernel(
   wait_for_predecessor();
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row0 = blockIdx.x * 32, row = row0 + lane;
-  float m = -INFINITY, s = 0.f;
-  if (row < R)
-    for (int i = w; i < slots; i += 8 * NW) {
-      float2 p[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        p[u] = i + u * NW < slots ? part[(size_t)(i + u * NW) * R + row] : make_float2(-INFINITY, 0.f);
-      float mn = m;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) mn = fmaxf(mn, p[u].x);
-      const float base = mn == -INFINITY ? 0.f : mn;
-      s *= expf((m - base) * inv_t);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) s += p[u].y * expf((p[u].x - base) * inv_t);
-      m = mn;
-    }
-  ms[w][lane] = make_float2(m, s);
-  __syncthreads();
+  float m, s, base;
+  join_slots<NW>(part, slots, R, inv_t, ms, m, s, base);
   if (w == 0) {
-#pragma unroll
-    for (int i = 1; i < NW; ++i) m = fmaxf(m, ms[i][lane].x);
-    const float base = m == -INFINITY ? 0.f : m;
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) s += ms[i][lane].y * expf((ms[i][lane].x - base) * inv_t);
     if (!sq) {
       if (row < R) {
         const int id = sid[row];
@@ -302,6 +326,22 @@ int piece_cols(int R, int V) {
   return (int)std::min<long long>(std::max<long long>(c, 256), ((long long)V + 255) / 256 * 256);
 }
 
+// Columns of one piece of the forward: statistics of at most 256 MB (64-column
+// slots), so that they stay a fixed amount of scratch whatever R V is. One piece
+// up to 2^31 logits; a further one costs a join and, for a soft target, a
+// launch of the lists.
+int stat_piece_cols(int R, int V) {
+  const long long c = (1ll << 31) / R / 256 * 256;  // 256 at the largest R
+  return (int)std::min<long long>(c, ((long long)V + 255) / 256 * 256);
+}
+
+// The start table of the target lists covers this many columns of the vocabulary
+// at a time (64 MB at most): whole pieces of the backward.
+int list_cols(int R, int V, bool backward) {
+  const int c = stat_piece_cols(R, V);
+  return backward ? c / piece_cols(R, V) * piece_cols(R, V) : c;
+}
+
 int num_slots(int V) { return (int)(((long long)V + 255) / 256 * (256 / kHeadSlot)); }
 
 struct Carve {
@@ -314,30 +354,43 @@ struct Carve {
   }
 };
 
-size_t list_bytes(int R, int V, int K) {
-  return 2 * align128((size_t)R * K * 4) + align128((size_t)R * 4) + align128((size_t)R * num_slots(V) * 2);
+size_t list_bytes(int R, int K, int cols) {
+  return 2 * align128((size_t)R * K * 4) + align128((size_t)R * 4) + align128((size_t)R * num_slots(cols) * 2);
 }
 
-// Sorted target lists of the soft target (the hard one is its own list).
-cudaError_t target_lists(const HeadArgs& a, Carve& c, HeadTcArgs& t, cudaStream_t s) {
+// Sorted target lists of the soft target (the hard one is its own list), with
+// the start table of the columns [c0, c0 + cols).
+struct Lists {
+  int *sid, cols;
+  float *q, *live;
+  uint16_t* start;
+};
+Lists carve_lists(const HeadArgs& a, Carve& c, int cols) {
+  Lists l{};
+  l.cols = cols;
+  if (!a.teacher) return l;
+  l.sid = c.take<int>((size_t)a.R * a.K);
+  l.q = c.take<float>((size_t)a.R * a.K);
+  l.live = c.take<float>(a.R);
+  l.start = c.take<uint16_t>((size_t)a.R * num_slots(cols));
+  return l;
+}
+cudaError_t target_lists(const HeadArgs& a, const Lists& l, int c0, HeadTcArgs& t, cudaStream_t s) {
   t.sid = a.idx;
   t.K = a.K;
   if (!a.teacher) return cudaSuccess;
-  int* si = c.take<int>((size_t)a.R * a.K);
-  float* q = c.take<float>((size_t)a.R * a.K);
-  float* live = c.take<float>(a.R);
-  t.slots = num_slots(a.V);
-  uint16_t* start = c.take<uint16_t>((size_t)a.R * t.slots);
-  t.sid = si;
-  t.sq = q;
-  t.live = live;
-  t.start = start;
+  t.slots = num_slots(l.cols);
+  t.slot0 = c0 / kHeadSlot;
+  t.sid = l.sid;
+  t.sq = l.q;
+  t.live = l.live;
+  t.start = l.start;
   auto kern = a.K <= 32    ? head_lists_kernel<1>
               : a.K <= 64  ? head_lists_kernel<2>
               : a.K <= 128 ? head_lists_kernel<4>
                            : head_lists_kernel<8>;
-  return launch_dependent(kern, (a.R + 3) / 4, 128, 0, 1, s, a.idx, a.teacher, a.R, a.V, a.K, a.inv_t, si, q, live, start,
-                          t.slots);
+  return launch_dependent(kern, (a.R + 3) / 4, 128, 0, 1, s, a.idx, a.teacher, a.R, a.V, a.K, a.inv_t, l.sid, l.q, l.live,
+                          l.start, t.slots, t.slot0);
 }
 
 HeadTcArgs tc_args(const HeadArgs& a) {
@@ -355,8 +408,10 @@ HeadTcArgs tc_args(const HeadArgs& a) {
 }  // namespace
 
 size_t head_fwd_scratch_bytes(int R, int V, int d, int K, bool lists) {
-  const int slots = std::max((V + 63) / 64, lists ? 0 : head_small_slots(R, V, d));
-  return align128((size_t)slots * R * 8) + align128((size_t)R * K * 4) + (lists ? list_bytes(R, V, K) : 0);
+  const int pc = stat_piece_cols(R, V), cols = head_stat_cols(d, true);  // a bias never widens the slots
+  const int slots = std::max((std::min(pc, V) + cols - 1) / cols + (pc < V), lists ? 0 : head_small_slots(R, V, d));
+  return align128((size_t)slots * R * 8) + align128((size_t)R * K * 4) +
+         (lists ? list_bytes(R, K, list_cols(R, V, false)) : 0);
 }
 
 // How the backward of one problem is cut: columns per piece, the slices of the
@@ -381,7 +436,8 @@ size_t head_bwd_scratch_bytes(int R, int V, int d, int K, bool lists) {
   const Plan p = make_plan(R, V, d);
   return align128((size_t)R * p.pc * 2) + align128((size_t)p.slabs * p.pc * 4) +
          align128(p.dh_scratch ? (size_t)p.sp.dh * R * p.dp * 4 : 0) +
-         align128(p.sp.dw > 1 ? (size_t)p.sp.dw * std::min(p.pc, V) * p.dp * 4 : 0) + (lists ? list_bytes(R, V, K) : 0);
+         align128(p.sp.dw > 1 ? (size_t)p.sp.dw * std::min(p.pc, V) * p.dp * 4 : 0) +
+         (lists ? list_bytes(R, K, list_cols(R, V, true)) : 0);
 }
 
 dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s) {
@@ -389,24 +445,39 @@ dgx_status head_fwd(const HeadArgs& a, void* ws, cudaStream_t s) {
   HeadTcArgs t = tc_args(a);
   const int small = a.teacher ? 0 : head_small_slots(a.R, a.V, a.d);
   const int cols = head_stat_cols(a.d, a.bias != nullptr);
-  const int slots = small ? small : (a.V + cols - 1) / cols;
-  t.part = c.take<float2>((size_t)slots * a.R);
+  const int pc = small ? a.V : stat_piece_cols(a.R, a.V);
+  const int first = pc < a.V;  // several pieces: slot 0 holds the joined earlier ones
+  const int max_slots = small ? small : (std::min(pc, a.V) + cols - 1) / cols + first;
+  float2* part = c.take<float2>((size_t)max_slots * a.R);
   t.zs = c.take<float>((size_t)a.R * a.K);
-  t.n = a.V;
+  const Lists lists = carve_lists(a, c, list_cols(a.R, a.V, false));
   const bool whole = !a.teacher && !small && a.V <= 256;  // one tile holds a row: finished in the tile's epilogue
   if (whole) {
     t.loss = a.loss;
     t.lse_out = a.lse;
   }
-  cudaError_t e = target_lists(a, c, t, s);
-  if (e == cudaSuccess)
-    e = small ? head_small(t, a.H, a.ldh, a.W, a.ldw, small, a.loss, a.lse, s)
-              : head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, false, nullptr, 0, s);
-  if (e == cudaSuccess && small != 1 && !whole) {
+  cudaError_t e = cudaSuccess;
+  for (int c0 = 0; c0 < a.V && e == cudaSuccess; c0 += pc) {
+    t.c0 = c0;
+    t.n = std::min(pc, a.V - c0);
+    t.part = part + (size_t)first * a.R;
+    e = target_lists(a, lists, c0, t, s);
+    if (e == cudaSuccess)
+      e = small ? head_small(t, a.H, a.ldh, a.W, a.ldw, small, a.loss, a.lse, s)
+                : head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, false, nullptr, 0, s);
+    if (e != cudaSuccess || small == 1 || whole) break;
+    const bool earlier = c0 > 0;
+    const float2* from = earlier ? part : t.part;
+    const int slots = (small ? small : (t.n + cols - 1) / cols) + earlier;
+    const unsigned blocks = (a.R + 31) / 32;
+    if (t.n < a.V - c0) {
+      e = launch_dependent(head_join_kernel, blocks, 1024, 0, 1, s, from, slots, a.R, a.inv_t, part);
+      continue;
+    }
     // few slots: few warps, so that many rows do not pay for idle ones
     const bool wide = slots > 32;
-    e = launch_dependent(wide ? head_finish_kernel<32> : head_finish_kernel<4>, (a.R + 31) / 32, wide ? 1024 : 128, 0, 1,
-                         s, t.part, slots, a.R, a.V, a.t, a.inv_t, t.sid, t.sq, a.K, t.zs, a.loss, a.lse);
+    e = launch_dependent(wide ? head_finish_kernel<32> : head_finish_kernel<4>, blocks, wide ? 1024 : 128, 0, 1, s, from,
+                         slots, a.R, a.V, a.t, a.inv_t, t.sid, t.sq, a.K, t.zs, a.loss, a.lse);
   }
   if (e == cudaSuccess && a.mean) e = launch_dependent(head_mean_kernel, 1, 1024, 0, 1, s, a.loss, a.R, a.mean);
   return cuda_status(e, "head forward");
@@ -426,8 +497,9 @@ dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
   float* dbp = c.take<float>((size_t)p.slabs * p.pc);
   float* dh = p.dh_scratch ? c.take<float>((size_t)p.sp.dh * a.R * p.dp) : nullptr;
   float* dw = p.sp.dw > 1 ? c.take<float>((size_t)p.sp.dw * std::min(p.pc, a.V) * p.dp) : nullptr;
-  cudaError_t e = target_lists(a, c, t, s);
-  if (e != cudaSuccess) return cuda_status(e, "head backward");
+  const int lc = list_cols(a.R, a.V, true);
+  const Lists lists = carve_lists(a, c, lc);
+  cudaError_t e = cudaSuccess;
   t.dbp = a.db ? dbp : nullptr;
   t.dloss = a.dloss;
   t.lse = a.lse;
@@ -435,7 +507,8 @@ dgx_status head_bwd(const HeadArgs& a, void* ws, cudaStream_t s) {
     const int n = std::min(p.pc, a.V - c0);
     t.c0 = c0;
     t.n = n;
-    e = head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, true, g, p.pc, s);
+    if (c0 % lc == 0) e = target_lists(a, lists, c0, t, s);
+    if (e == cudaSuccess) e = head_logits_tc(t, a.H, a.ldh, a.W, a.ldw, true, g, p.pc, s);
     if (e != cudaSuccess) return cuda_status(e, "head backward");
     HeadGradTc m{};
     m.G = g;

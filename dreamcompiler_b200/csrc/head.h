@@ -48,11 +48,11 @@ struct HeadTcArgs {
   const float* bias;        // [V] or null
   const int* sid;           // [R][K] target ids, ascending when K > 1
   const float* sq;          // [R][K] their probabilities, or null (1)
-  const uint16_t* start;    // [R][slots] first entry with id >= kHeadSlot * slot, or null (K = 1)
-  int slots;
+  const uint16_t* start;    // [R][slots] first entry with id >= kHeadSlot * (slot0 + slot), or null (K = 1)
+  int slots, slot0;
   float* zs;                // [R][K] out: raw logits at the ids (statistics)
                             // (a hard target's is left out of the row's statistics)
-  float2* part;             // [ceil(n / head_stat_cols())][R] out: (max, sum) per slot of columns (statistics)
+  float2* part;             // [ceil(n / head_stat_cols())][R] out: (max, sum) per slot of the piece's columns (statistics)
   float *loss, *lse_out;    // [R] out: a hard target's results where one tile holds every column
                             // (n = V <= 256; zs and part are not written then), or null (statistics)
   const float* live;        // [R] 0 where the row has no target, or null (id in [0, V))

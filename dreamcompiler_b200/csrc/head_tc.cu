@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(64 + 32 * HD_EPI_WARPS, 1)
         tg.ids = a.sid + (size_t)row * a.K;
         tg.qs = a.sq ? a.sq + (size_t)row * a.K : nullptr;
         tg.K = a.K;
-        tg.start(a.start ? a.start[(size_t)row * a.slots + (a.c0 + nbase) / kHeadSlot] : 0);
+        tg.start(a.start ? a.start[(size_t)row * a.slots + (a.c0 + nbase) / kHeadSlot - a.slot0] : 0);
         if (MODE == kGrad) {
           const bool live = a.live ? a.live[row] != 0.f : (tg.nid >= 0 && tg.nid < a.V);
           w = live ? (a.dloss ? a.dloss[row] : 1.f) : 0.f;

@@ -122,6 +122,20 @@ def test_workspace_sizes(lib):
         assert lib.dgx_linear_distill_workspace_size(64, 1000, 64, 8, b) >= small
 
 
+@pytest.mark.parametrize("R,V,d", [(65536, 262144, 4096), (65536, 262144, 256), (16384, 1 << 23, 64), (1 << 23, 65, 64),
+                                   (3, 1 << 23, 2048), (300000, 100000, 1024)])
+def test_forward_workspace_does_not_grow_with_the_logits(lib, R, V, d):
+    """Statistics of 2^31 logits at a time (8 bytes for 64 or, from d = 769 on, 128 of them) and a start table of 2 bytes
+    for 64; beside that only K ids, probabilities and logits per row."""
+    for K in (1, 20):
+        rows = R * (12 * K + 16) + 4096
+        stats = (8 << 31) // (128 if d > 768 else 64)
+        assert lib.dgx_linear_nll_workspace_size(R, V, d, 0) <= stats + rows
+        assert lib.dgx_linear_distill_workspace_size(R, V, d, K, 0) <= stats + (2 << 31) // 64 + rows
+        extra = (lib.dgx_linear_distill_workspace_size(R, V, d, K, 1) - lib.dgx_linear_nll_workspace_size(R, V, d, 1))
+        assert 0 <= extra <= (2 << 31) // 64 + rows
+
+
 def test_faults_can_be_injected(lib):
     from dreamcompiler_b200 import _lib as L
     try:

@@ -535,3 +535,55 @@ def test_workspace_must_be_on_the_device(dgx):
                      lambda: dgx.linear_distill_bwd(H, H, i1, q1, row, workspace=bad)):
             with pytest.raises(AssertionError, match="workspace"):
                 call()
+
+
+def rows_of(p, K, r0, r1):
+    """The rows [r0, r1) of a problem that was made without its 64-bit results, with them."""
+    b = Problem.__new__(Problem)
+    b.__dict__.update(p, R=r1 - r0, K=K, dloss=None, H=p["H"][r0:r1])
+    if K is None:
+        b.target = p["target"][r0:r1]
+    else:
+        b.idx, b.teacher = p["idx"][r0:r1], p["teacher"][r0:r1]
+    b._truth()
+    return b
+
+
+@pytest.mark.parametrize("R,V,K", [(9000, 262144, None), (9000, 262144, 5), (1100, 2000003, 3), (70000, 31000, None)])
+def test_more_logits_than_one_forward_piece(dgx, R, V, K):
+    """Above 2^31 logits the forward joins the statistics of several pieces of the vocabulary, and the target lists'
+    start table is made anew for each (in the backward for each group of pieces)."""
+    g = torch.Generator(device="cuda").manual_seed(R)
+    rand = lambda *s: torch.rand(*s, device="cuda", generator=g)  # noqa: E731
+    d, T = 16, 1.0 if K is None else 2.0
+    W = torch.randn(V, d, device="cuda", generator=g) * 0.75
+    lead = torch.randint(0, V, (R,), device="cuda", generator=g)
+    H = (torch.randn(R, d, device="cuda", generator=g) + W[lead] * rand(R, 1)).bfloat16()
+    bias = torch.randn(V, device="cuda", generator=g)
+    p = dict(V=V, d=d, T=T, scale=1.0 / R, H=H, W=W.bfloat16(), bias=bias)
+    if K is None:
+        p["target"] = torch.where(rand(R) < 0.1, torch.full_like(lead, -1), lead).to(torch.int32)
+        call, args = (dgx.linear_nll_fwd, dgx.linear_nll_bwd), (p["target"],)
+        kw = dict(bias=bias)
+    else:
+        p["idx"] = torch.randint(-V // 20, V, (R, K), device="cuda", generator=g).to(torch.int32)
+        p["idx"][:, 0] = lead
+        p["teacher"] = 6.0 - 7.0 * rand(R, K)
+        call, args = (dgx.linear_distill_fwd, dgx.linear_distill_bwd), (p["idx"], p["teacher"])
+        kw = dict(bias=bias, temperature=T)
+    loss, lse = call[0](H, p["W"], *args, **kw)
+    dH, dW = torch.empty(R, d, device="cuda"), torch.empty(V, d, device="cuda")
+    _, _, db = call[1](H, p["W"], *args, lse, scale=1.0 / R, dH=dH, dW=dW, **kw)
+    dgx.sync_check()
+    total = {k: 0.0 for k in ("dW", "tol_dW", "db", "tol_db")}
+    step = max(1, (1 << 28) // V)
+    blocks = (R + step - 1) // step
+    for r0 in range(0, R, step):
+        b = rows_of(p, K, r0, min(R, r0 + step))
+        b.check_fwd(loss[r0:r0 + step], lse[r0:r0 + step])
+        b.check_bwd(dH[r0:r0 + step], None, None)
+        for k in total:
+            total[k] = total[k] + getattr(b, k)
+    # a block's bound counts the additions of its own rows: all R of them are at most `blocks` times as many
+    within(dW, total["dW"], blocks * total["tol_dW"], "dW")
+    within(db, total["db"], blocks * total["tol_db"], "db")

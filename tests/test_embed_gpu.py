@@ -204,3 +204,47 @@ def test_workspace_must_be_on_the_device(dgx):
     for bad in (torch.empty(1 << 20), torch.empty(1, device="cuda").expand(1 << 20)):
         with pytest.raises(AssertionError, match="workspace"):
             dgx.embed_bwd(tok, dx, 10, workspace=bad)
+
+
+@pytest.mark.parametrize("n,V,d", [(100, 262144, 40), (129, 262144, 24), (5000, 262144, 24), (70000, 262144, 17),
+                                   (3000, (1 << 27) + 5, 2)])
+@pytest.mark.parametrize("kind", ["spread", "hot", "invalid"])
+def test_backward_of_a_large_vocabulary(dgx, n, V, d, kind):
+    """Three and four passes of the sort (keys of 19 and 28 bits): the order ends in the other buffer, or in one that was
+    read before."""
+    g = torch.Generator(device="cuda").manual_seed(n + d)
+    tok = tokens(n, V, kind, g)
+    tok[::7] = torch.randint(0, 50, (tok[::7].numel(),), device="cuda", generator=g).to(torch.int32) * (V // 50)
+    dx = torch.randn(n, d, device="cuda", generator=g)
+    out = torch.full((V, d), float("nan"), device="cuda")
+    got = dgx.embed_bwd(tok, dx, V, scale=0.3, out=out)
+    ref, mag, cnt = truth(tok, dx, V, 0.3)
+    tol = U * (cnt[:, None] + 2) * mag + U * ref.abs()
+    assert ((got.to(F64) - ref).abs() <= tol + 1e-45).all()
+    assert not got[cnt == 0].any()
+
+
+@pytest.mark.parametrize("n", [1, 100, 128, 129, 4097])
+@pytest.mark.parametrize("V,d", [(70, 40), (500, 264), (300, 33)])
+@pytest.mark.parametrize("pad,off", [(0, 0), (3, 1), (8, 8)])
+@pytest.mark.parametrize("gx", ["f32", "bf16"])
+def test_backward_accumulates_into_pitched_rows(dgx, n, V, d, pad, off, gx):
+    """With and without the sort: rows that occur are added to, the others and the padding are left alone; the same
+    places without accumulate."""
+    g = torch.Generator(device="cuda").manual_seed(n + V + d)
+    tok = tokens(n, V, "hot", g)
+    dx = torch.randn(n, d + pad + off, device="cuda", generator=g).to(DT[gx])[:, off:off + d]
+    ref, mag, cnt = truth(tok, dx, V, 2.0)
+    hit = cnt > 0
+    tol = U * (cnt[:, None] + 4) * mag
+    for accumulate in (True, False):
+        base = torch.randn(V, d + pad + off, device="cuda", generator=g)
+        base[~hit] = float("nan")
+        buf = base.clone()
+        got = dgx.embed_bwd(tok, dx, V, scale=2.0, out=buf[:, off:off + d], accumulate=accumulate)
+        was = base[:, off:off + d].to(F64) if accumulate else torch.zeros(V, d, dtype=F64, device="cuda")
+        assert ((got.to(F64) - ref - was).abs() <= tol + U * 4 * was.abs())[hit].all()
+        assert got[~hit].isnan().all() if accumulate else not got[~hit].any()
+        keep = torch.ones(V, d + pad + off, dtype=torch.bool, device="cuda")
+        keep[:, off:off + d] = False
+        assert torch.equal(buf[keep].nan_to_num(7.0), base[keep].nan_to_num(7.0))

@@ -587,3 +587,63 @@ def test_more_logits_than_one_forward_piece(dgx, R, V, K):
     # a block's bound counts the additions of its own rows: all R of them are at most `blocks` times as many
     within(dW, total["dW"], blocks * total["tol_dW"], "dW")
     within(db, total["db"], blocks * total["tol_db"], "db")
+
+
+def masked_distillation(R, V, d, K, T, seed, masked_entries):
+    """Columns of -inf and of the lowest float; the teacher's entries there are absent, or present with a logit of -inf."""
+    p = Problem(R, V, d, K=K, T=T, bias="masked", absent=0.1, seed=seed, scale=1.0 / R, weighted=True)
+    off = (p.idx >= 0) & (p.bias[p.idx.clamp(min=0).long()] < -1e30)
+    if masked_entries == "absent":
+        p.idx[off] = -1
+    else:
+        p.teacher[off] = float("-inf")
+        p.teacher[(p.idx >= 0).any(1) & ~((p.idx >= 0) & ~off).any(1)] = 0.0  # no row of -inf entries alone ...
+        p.idx[off & (p.teacher > -1e30)] = -1  # ... whose masked ids leave instead
+    p._truth()
+    return p
+
+
+@pytest.mark.parametrize("R,V,d", [(2, 65, 384), (64, 257, 64), (129, 300, 72), (33, 8209, 256), (700, 2049, 40),
+                                   (1000, 65, 384)])
+@pytest.mark.parametrize("K,T", [(1, 1.0), (20, 0.25), (64, 4.0), (256, 2.0)])
+@pytest.mark.parametrize("masked_entries", ["absent", "-inf"])
+def test_distill_with_masked_columns(dgx, R, V, d, K, T, masked_entries):
+    """Masked columns have probability 0 whatever 1 / T makes of their logits; rows weighted."""
+    p = masked_distillation(R, V, d, K, T, R + V + K, masked_entries)
+    off = p.bias < -1e30
+    assert off.any() or R > 8 * V  # so many rows that every column leads one, and none may be masked
+    loss, lse = p.fwd(dgx)
+    p.check_fwd(loss, lse)
+    dH, dW, db = p.bwd(dgx, lse)
+    p.check_bwd(dH, dW, db)
+    assert not dW[off].any() and not db[off].any()
+
+
+@pytest.mark.parametrize("T", [0.125, 0.5, 30.0])
+@pytest.mark.parametrize("R,V,d,K", [(5, 300, 64, 8), (300, 1000, 136, 33)])
+def test_distill_temperatures_and_row_weights(dgx, R, V, d, K, T):
+    p = Problem(R, V, d, K=K, T=T, bias="plain", absent=0.2, weighted=True, seed=R + K, scale=1.0 / R)
+    loss, lse = p.fwd(dgx)
+    p.check_fwd(loss, lse)
+    p.check_bwd(*p.bwd(dgx, lse))
+
+
+@pytest.mark.parametrize("R,V,d,bias", [(9, 65, 384, None), (16, 65, 384, "masked"), (10, 5003, 1000, "plain"),
+                                        (13, 300, 20, "masked"), (16, 20011, 1024, None), (17, 5003, 1000, "plain"),
+                                        (8, 5003, 1000, "plain"), (15, 2049, 3000, "plain"), (16, 777, 3080, None)])
+def test_few_rows_of_ordinary_values(dgx, R, V, d, bias):
+    """Both row groups of the thin kernel (up to 16 rows, while their fragments fit shared memory) and what follows it."""
+    p = Problem(R, V, d, bias=bias, ignored=0.2, seed=R + V, scale=1.0 / R)
+    loss, lse = p.fwd(dgx)
+    p.check_fwd(loss, lse)
+    p.check_bwd(*p.bwd(dgx, lse))
+
+
+@pytest.mark.parametrize("K", [None, 40])
+@pytest.mark.parametrize("R,V,d", [(100, 500, 2048), (520, 1300, 2000), (7, 300, 4104)])
+def test_long_contractions(dgx, R, V, d, K):
+    p = Problem(R, V, d, K=K, T=1.0 if K is None else 2.0, bias="plain", ignored=0.1, absent=0.1, weighted=True, seed=d,
+                scale=1.0 / R)
+    loss, lse = p.fwd(dgx)
+    p.check_fwd(loss, lse)
+    p.check_bwd(*p.bwd(dgx, lse))

@@ -696,8 +696,13 @@ int wide_cluster() {
 
 cudaError_t launch_sort(const SortArgs& a, cudaStream_t s) {
   const int wide = wide_cluster();
-  // up to 4096 tokens one CTA sorts without leaving its SM
-  const int cluster = a.n <= 4096 ? 1 : a.n <= 8192 ? 8 : wide;
+  // Up to 2048 tokens one CTA sorts without leaving its SM, up to 8192 a cluster
+  // of 8. The whole gradient with 1, 8 and 16 CTAs, tables of 1000 x 64 and
+  // 50257 x 64 (us): 1000 tokens 14.7, 16.7, 16.8 and 14.9, 17.5, 18.5; 2048
+  // tokens 17.0, 17.0, 17.3 and 18.3, 18.2, 19.3; 4096 tokens 21.8, 17.5, 17.9 and
+  // 24.3, 19.1, 19.9; 8192 tokens 32.7, 17.5, 17.8 and 39.1, 20.9, 21.5; 8193
+  // tokens 34.4, 19.7, 17.9 and 40.9, 23.3, 21.6.
+  const int cluster = a.n <= 2048 ? 1 : a.n <= 8192 ? 8 : wide;
   return launch_dependent(embed_sort_kernel, cluster, kSortThreads, kSortWarps * 4 << a.bits, cluster, s, a);
 }
 

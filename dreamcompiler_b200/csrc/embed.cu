@@ -160,7 +160,10 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const int* __restrict__ 
 // per item and SM: 65536 ids of 18 bits (two passes) take 26 us on 16 CTAs, 41
 // on 8; 16384 ids of 7 bits (one pass) 7 us.
 constexpr int kSortThreads = 1024, kSortWarps = 32, kMaxDigitBits = 9, kMaxCluster = 16;
-constexpr int kBatch = 4;  // keys per lane in registers (65536 keys in 16 CTAs)
+// Keys per lane in registers: 65536 keys in 16 CTAs. Beyond, keys are read twice
+// and ranks go through memory (whole gradient on 1000 x 64: 65536 tokens 29.4
+// us, 65537 34.3, 131072 51.6).
+constexpr int kBatch = 4;
 
 struct SortArgs {
   const int* tok;
@@ -320,7 +323,8 @@ struct SumArgs {
   int n, d, V, slabs, blocks;
   int lddx, lddw, accumulate;
   float scale;
-  int zero_blocks, bulk;  // blocks that zero rows; rows of dW are whole aligned 16-byte units
+  int zero_blocks, zero_rows;  // blocks that zero rows, and rows for each
+  int bulk;                    // rows of dW are whole aligned 16-byte units
 };
 
 template <typename TW, bool VEC>
@@ -401,11 +405,10 @@ __device__ __forceinline__ void put_part(const SumArgs& a, SumShared& sh, int bl
 // out as bulk copies of a zeroed piece of shared memory. These blocks come
 // first: the sums' latency hides behind their writes (gradient of 16381 tokens
 // on 50257 x 1024 fp32 59 us, 62 with them last; 4096 on 32768 x 1024 47
-// against 53; 65536 on 131072 x 2048 bf16 161.5 against 160). 32, 64 or 256 rows
-// a block: 61, 64 and 63 us for the first of these. A launch of its own beside
+// against 53; 65536 on 131072 x 2048 bf16 161.5 against 160). A launch of its own beside
 // the sort took 52, but would have to read the ids and write dW without having
 // waited for the work before the call.
-constexpr int kZeroRows = 128;
+constexpr int kZeroRows = 128, kZeroBytes = 64 << 10;
 
 template <typename TW>
 __device__ __forceinline__ void zero_rows(const SumArgs& a, SumShared& sh, TW* dW, unsigned group) {
@@ -415,32 +418,37 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, SumShared& sh, TW* d
     fence_proxy_async_smem();
   }
   __syncthreads();
-  const unsigned t = group * kZeroRows + w * (kZeroRows / 8) + lane;
-  bool absent = lane < kZeroRows / 8 && t < (unsigned)a.V;
-  if (absent) {
-    int lo = 0, hi = a.n;  // first position whose token is t or above
-    while (lo < hi) {
-      const int mid = lo + (hi - lo) / 2;
-      if ((unsigned)a.sorted[mid].x < t)
-        lo = mid + 1;
-      else
-        hi = mid;
+  const int each = min(a.zero_rows, 256) / 8;  // rows per warp and pass
+  for (int r = 0; r < a.zero_rows; r += 256) {
+    const unsigned t = group * a.zero_rows + r + w * each + lane;
+    bool absent = lane < each && t < (unsigned)a.V;
+    if (absent) {
+      int lo = 0, hi = a.n;  // first position whose token is t or above
+      while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if ((unsigned)a.sorted[mid].x < t)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      absent = lo == a.n || (unsigned)a.sorted[lo].x != t;
     }
-    absent = lo == a.n || (unsigned)a.sorted[lo].x != t;
+    if (a.bulk) {
+      const int bytes = a.d * (int)sizeof(TW);
+      char* row = reinterpret_cast<char*>(dW + (size_t)t * a.lddw);
+      if (absent)
+        for (int j = 0; j < bytes; j += (int)sizeof(sh.head))
+          bulk_store(row + j, sh.head, (uint32_t)min((int)sizeof(sh.head), bytes - j));
+    } else {
+      for (unsigned m = __ballot_sync(0xffffffffu, absent); m; m &= m - 1) {
+        TW* row = dW + (size_t)(t - lane + __ffs(m) - 1) * a.lddw;
+        for (int j = lane; j < a.d; j += 32) row[j] = TW(0.f);
+      }
+    }
   }
   if (a.bulk) {
-    const int bytes = a.d * (int)sizeof(TW);
-    char* row = reinterpret_cast<char*>(dW + (size_t)t * a.lddw);
-    if (absent)
-      for (int j = 0; j < bytes; j += (int)sizeof(sh.head))
-        bulk_store(row + j, sh.head, (uint32_t)min((int)sizeof(sh.head), bytes - j));
     bulk_commit();
     bulk_wait0();
-  } else {
-    for (unsigned m = __ballot_sync(0xffffffffu, absent); m; m &= m - 1) {
-      TW* row = dW + (size_t)(t - lane + __ffs(m) - 1) * a.lddw;
-      for (int j = lane; j < a.d; j += 32) row[j] = TW(0.f);
-    }
   }
 }
 
@@ -559,11 +567,12 @@ __global__ void __launch_bounds__(256, 4) embed_sum_kernel(const TG* __restrict_
 // ---------------------------------------------------------------- few tokens
 // Up to kFew tokens need no sort: a block owns 32 table rows, reads all ids,
 // keeps those of its rows in order, and each warp sums and writes (or zeroes)
-// 256 columns of four rows. One launch instead of three: 100 ids on 5000 x 1024
-// fp32 7 us instead of 12.5. The rows of one token are added by one warp, which
-// bounds kFew (128 equal ids there: 17 us); a table of more than kFewBytes is
-// zeroed faster by the bulk copies of the sorted form (128 ids on 50257 x 768
-// fp32: 40 us against 36).
+// 256 columns of four rows. One launch instead of two: 128 ids on 5000 x 1024
+// fp32 7 us instead of 17. The rows of one token are added by one warp, which
+// bounds kFew, and kFewBytes lies where equal ids begin to lose what spread ones
+// gain (128 ids, this against the sorted form, us: spread and all equal, 20 MB
+// of table 7.3 / 17.2 and 18.9 / 17.5; 29 MB 9.6 / 17.7 and 26 / 17.9; 49 MB 14.5
+// / 18.2 and 38 / 18.4; 154 MB 40 / 35 and 63 / 35).
 constexpr int kFew = 128;
 constexpr long long kFewBytes = 32ll << 20;
 
@@ -706,6 +715,19 @@ cudaError_t launch_sort(const SortArgs& a, cudaStream_t s) {
   return launch_dependent(embed_sort_kernel, cluster, kSortThreads, kSortWarps * 4 << a.bits, cluster, s, a);
 }
 
+// Rows of dW for one block to look up and zero: three blocks for an SM, which
+// leaves room for the sums, but not more rows than 128 or 64 KB. Whole gradient
+// (us) by rows per block: 16381 tokens on 50257 x 1024 fp32 61 at 32, 64 at 64, 59
+// at 128 and 63 at 256; 200 on 5000 x 1024 17.2 at 16 and 18.6 at 128; 1000 on
+// 20000 x 1024 27.9 at 64 and 31.4 at 128; 300 on 1000000 x 16 49 at 128, 36.6 at
+// 256 and 31.7 at 1024.
+int zero_rows_per_block(int V, size_t row_bytes) {
+  const long long most = std::max<long long>(kZeroRows, kZeroBytes / (long long)row_bytes);
+  int rows = 16;
+  while (2ll * rows <= most && V > 3ll * num_sms() * rows) rows *= 2;
+  return rows;
+}
+
 template <typename TG, typename TW, bool VEC>
 cudaError_t launch_sum(const int* tok, const void* dx, void* dW, const SumArgs& a, int blocks, bool few, cudaStream_t s) {
   if (few) {
@@ -777,7 +799,8 @@ dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int 
     return cuda_status(cudaMemset2DAsync(dW, lddw * es, 0, d * es, V, s), "dgx_embed_bwd");
   }
   const Layout l = layout(n, d, V);
-  const long long zero_blocks = ((long long)V + kZeroRows - 1) / kZeroRows;
+  const int zero_rows = zero_rows_per_block(V, (size_t)d * type_size(dw_type));
+  const long long zero_blocks = ((long long)V + zero_rows - 1) / zero_rows;
   if ((long long)l.blocks * l.slabs + zero_blocks > 0x7fffffffll || l.slabs > 65535)
     return set_error(DGX_EINVAL, "dgx_embed_bwd: n=%d V=%d d=%d too large", n, V, d);
   char* ws = (char*)workspace;
@@ -818,6 +841,7 @@ dgx_status dgx_embed_bwd(const int* tok, const void* dx, dgx_dtype dx_type, int 
     a.parts = (float*)(ws + l.parts);
     const size_t ts = type_size(dw_type);
     a.zero_blocks = accumulate ? 0 : (int)zero_blocks;
+    a.zero_rows = zero_rows;
     a.bulk = (((uintptr_t)dW | lddw * ts | d * ts) & 15) == 0;
   }
   const int blocks = l.blocks * l.slabs + a.zero_blocks;

@@ -43,7 +43,8 @@ dgx_status cuda_status(cudaError_t e, const char* what);
 // split-K partial tiles (kScratchSplitK) while its operands may sit in the
 // general buffer (the 3xTF32 planes); the convolution's im2col matrices
 // (kScratchConv) while its GEMMs use both; the vocabulary head's piece of
-// gradients and partial statistics (kScratchHead) while its GEMMs split K.
+// gradients, partial statistics and slices (kScratchHead; the embedding's sort
+// beside it takes the general buffer).
 constexpr int kScratchGeneral = 0, kScratchSplitK = 1, kScratchConv = 2, kScratchHead = 3, kScratchSlots = 4;
 void* library_scratch_slot(int slot, size_t bytes, cudaStream_t s);
 void* library_scratch(size_t bytes, cudaStream_t s);  // the general slot

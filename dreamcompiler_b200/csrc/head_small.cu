@@ -7,9 +7,11 @@
 // H is laid out in shared memory in the same order (the order of a sum's terms
 // is free), so nothing is staged or transposed.
 //
-// R = 1, V = 32768, d = 1024 (67 MB of W) takes 20 us a call, bound by the
-// stream of W. The tcgen05 kernel takes 33: its 256-row tiles are 128 tiles for 74
-// SM pairs and keep a few stages of loads in flight.
+// Bound by the stream of W where W is large: 131072 x 2048 (537 MB) takes 96 us
+// for one row, 5.6 TB/s. 32768 x 1024 (67 MB) takes 18.4 us, 3.6 TB/s: 256 blocks
+// of one tile per warp, unevenly on 148 SMs, then the kernel that joins their
+// statistics. The tcgen05 kernel, whose 256-row tiles keep a few stages of loads
+// in flight on 74 SM pairs, takes 149 and 28 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -172,6 +174,10 @@ int small_smem(int R, int d) { return (d + 31) / 32 * ((R + 7) / 8) * 512; }
 
 // Statistics slots (blocks) of the small kernel, 0 where it does not apply: up
 // to 16 rows whose fragments fit 96 KB of shared memory (two blocks per SM).
+// Small against tcgen05 kernel, whole forward (us), at 8, 16 and, by the latter
+// alone, 17 rows: 32768 x 1024 19.2 / 25.3, 22.6 / 23.5, 23.7; 131072 x 2048
+// 98 / 138, 103 / 133, 133; 5000 x 512 7.2 / 10.7, 8.4 / 11.0, 10.9; 65 x 384
+// 4.0 / 7.4, 4.7 / 7.4, 7.4.
 int head_small_slots(int R, int V, int d) {
   if (R > 16 || small_smem(R, d) > 96 * 1024) return 0;
   const int tiles = (V + kTileRows - 1) / kTileRows;

@@ -400,12 +400,12 @@ __device__ __forceinline__ void put_part(const SumArgs& a, SumShared& sh, int bl
 
 // ---------------------------------------------------------------- rows without a token
 // Blocks of the summing launch zero the rows of dW whose token does not occur,
-// kZeroRows rows each: a lane looks its row up in the sorted tokens (all rows
-// at once, so the search's dependent loads cost a few us in all) and sends it
-// out as bulk copies of a zeroed piece of shared memory. These blocks come
+// up to 256 rows at a time: a lane looks its row up in the sorted tokens (all
+// rows at once, so the search's dependent loads cost a few us in all) and sends
+// it out as bulk copies of a zeroed piece of shared memory. These blocks come
 // first: the sums' latency hides behind their writes (gradient of 16381 tokens
-// on 50257 x 1024 fp32 59 us, 62 with them last; 4096 on 32768 x 1024 47
-// against 53; 65536 on 131072 x 2048 bf16 161.5 against 160). A launch of its own beside
+// on 50257 x 1024 fp32 59 us, 62 with them last; 4096 on 32768 x 1024 47 against
+// 53; 65536 on 131072 x 2048 bf16 161.5 against 160). A launch of its own beside
 // the sort took 52, but would have to read the ids and write dW without having
 // waited for the work before the call.
 constexpr int kZeroRows = 128, kZeroBytes = 64 << 10;
